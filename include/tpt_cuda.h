@@ -50,7 +50,12 @@ typedef enum tpt_status {
 } tpt_status;
 
 /* Epilogue activation (the Relu / Gelu nodes of exec.rs:416-445, fused). */
-typedef enum tpt_act { TPT_ACT_NONE = 0, TPT_ACT_RELU = 1, TPT_ACT_GELU = 2 } tpt_act;
+typedef enum tpt_act {
+    TPT_ACT_NONE = 0,
+    TPT_ACT_RELU = 1,
+    TPT_ACT_GELU = 2,
+    TPT_ACT_SILU = 3 /* x / (1 + e^-x); only the 16-bit products below take it */
+} tpt_act;
 
 typedef struct tpt_cuda_ctx tpt_cuda_ctx;
 typedef struct tpt_cuda_weights tpt_cuda_weights;
@@ -303,7 +308,8 @@ int tpt_cuda_w4_gemm_dev(tpt_cuda_ctx *ctx, const float *x, size_t m, const tpt_
  * (crates/tpt-infer-quantize/src/quant.rs:25-31). */
 typedef struct tpt_cuda_plan tpt_cuda_plan;
 
-enum { TPT_DT_F32 = 0, TPT_DT_I8 = 1 };
+/* plan tensors are F32 or I8; the 16-bit types are those of the products below */
+enum { TPT_DT_F32 = 0, TPT_DT_I8 = 1, TPT_DT_BF16 = 2, TPT_DT_F16 = 3 };
 
 enum tpt_op_kind {
     TPT_OP_QUANTIZE = 1,        /* in0 f32 [d0] -> out i8, per-tensor scale; d1 != 0: the calibration max is
@@ -401,6 +407,61 @@ int tpt_cuda_plan_run(tpt_cuda_plan *plan, const int *in_ids, const float *const
  * runs. Returns after the last outputs are in host memory. */
 int tpt_cuda_plan_run_batches(tpt_cuda_plan *plan, const int *in_ids, const float *const *inputs, size_t n_in,
                               const int *out_ids, float *const *outputs, size_t n_out, size_t n_steps);
+
+/* ------------------------------------------------------------------ */
+/* 16-bit products and mixture-of-experts layers                        */
+/* ------------------------------------------------------------------ */
+
+/* No counterpart in the reference (f32, INT8 and INT4 only): the layers of
+ * models whose weights stay in bf16 or f16. Operands are TPT_DT_BF16 or
+ * TPT_DT_F16 (16-bit words); every sum and epilogue is in f32, rounded once to
+ * the output's type. Device pointers, async on the context's stream; strides
+ * count elements. Outputs must not overlap inputs, except that `residual` may
+ * be `y` itself. Errors: TPT_UNSUPPORTED for another type or a size past the
+ * limits, TPT_SHAPE_MISMATCH for a stride shorter than its row, TPT_INVALID
+ * for anything else (null or misaligned pointers, unknown enum values). */
+
+/* y[m, n] = act(x[m, k] w[n, k]^T + bias[n]) + residual[m, n]. bias (of the
+ * operands' type) and residual (of y's type) may be NULL; y_dtype is the
+ * operands' type or TPT_DT_F32. k = 0 gives act(bias) + residual. */
+int tpt_cuda_linear_dev(tpt_cuda_ctx *ctx, int dtype, const void *x, size_t ldx, size_t m, size_t k, const void *w,
+                        size_t ldw, size_t n, const void *bias, int act, const void *residual, size_t ldr, void *y,
+                        size_t ldy, int y_dtype);
+
+/* Routing of tokens to experts. logits [tokens, experts] (f32, bf16 or f16,
+ * rows ld apart); s = softmax or sigmoid of a token's logits in f32. Experts
+ * are ordered by s + bias (bias [experts] f32 or NULL), ties by the lowest
+ * index. With groups > 1 the experts form `groups` equal contiguous groups; a
+ * group's score is the sum of its group_top (1 or 2) best s + bias, and only
+ * the groups_kept best groups (ties: lowest index) stay. The top_k best
+ * experts' indices go to ids [tokens, top_k], best first, their s (without the
+ * bias) to weights, divided by their sum if renormalise, times scale.
+ * A logit of -inf or NaN (or such a bias) takes its expert out; where fewer
+ * than top_k experts are left, the rest of ids is -1 with weight 0, and so is
+ * every entry of a token whose mask byte is 0 (mask [tokens] or NULL).
+ * top_k must not exceed the experts of groups_kept groups. */
+typedef enum tpt_score { TPT_SCORE_SOFTMAX = 0, TPT_SCORE_SIGMOID = 1 } tpt_score;
+#define TPT_ROUTE_MAX_EXPERTS 1024
+#define TPT_ROUTE_MAX_TOP_K 32
+int tpt_cuda_route_experts_dev(tpt_cuda_ctx *ctx, const void *logits, int dtype, size_t ld, size_t tokens,
+                               size_t experts, int score, const float *bias, size_t groups, size_t groups_kept,
+                               size_t group_top, size_t top_k, int renormalise, float scale, const uint8_t *mask,
+                               int32_t *ids, float *weights);
+
+/* The experts' feed-forward layers: y[t, :] = residual[t, :] +
+ * sum_j weights[t, j] W_out[e] h with e = ids[t, j], h = act(W_in[e] x[t, :]),
+ * or with `gated` h = act(g) * u, (g; u) = W_in[e] x[t, :] (elementwise
+ * product). w_in is [experts, f (gated: 2 f, the rows of g first), d], w_out
+ * [experts, d, f], both dense; ids and weights [tokens, top_k] as
+ * tpt_cuda_route_experts_dev writes them (a negative id is no expert; an id
+ * past the last expert counts as none and makes the next synchronising call
+ * return TPT_DEVICE_CHECK). h is rounded to the operands' type between the
+ * two products; the sum over j is in f32, in the order of j. */
+#define TPT_EXPERTS_MAX 4096
+int tpt_cuda_experts_mlp_dev(tpt_cuda_ctx *ctx, int dtype, const void *x, size_t ldx, size_t tokens, size_t d,
+                             const int32_t *ids, const float *weights, size_t top_k, const void *w_in,
+                             const void *w_out, size_t experts, size_t f, int act, int gated, const void *residual,
+                             size_t ldr, void *y, size_t ldy);
 
 /* ------------------------------------------------------------------ */
 /* Multi-GPU (one process per GPU on one node)                          */

@@ -1,0 +1,271 @@
+"""The 16-bit matrix product with its epilogue, against the formula in 64 bits.
+
+Bounds. The operands are exact in 64 bits, products of two 16-bit values are
+exact in f32, so a kernel's error is: the f32 sum's, at most (k + 2) 2^-23 S
+with S = sum |x w| + |bias| (also for truncating adders); the activation's,
+whose slope is at most 1.13 and whose own error is at most 4e-6 (1 + |value|);
+the residual's addition, 2^-23 of the terms; and the rounding to the output's
+type, 2^-8 (bf16) or 2^-11 (f16) of the result, plus f16's smallest step.
+"""
+import ctypes as C
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+ROUND = {"bf16": 2.0**-8, "f16": 2.0**-11, "f32": 2.0**-24}
+STEP = {"bf16": 1e-40, "f16": 2.0**-24, "f32": 1e-40}
+
+
+def _types():
+    import torch
+
+    return {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def act64(v, act):
+    import torch
+
+    if act == "relu":
+        return v.clamp(min=0)
+    if act == "gelu":
+        return 0.5 * v * (1 + torch.tanh(0.7978845608028654 * (v + 0.044715 * v**3)))
+    if act == "silu":
+        return v * torch.sigmoid(v)
+    return v
+
+
+def want(x, w, bias, act, residual, out_type):
+    """(y, bound) in 64 bits."""
+    xd, wd = x.double(), w.double()
+    k = x.shape[1]
+    v, s = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    if bias is not None:
+        v, s = v + bias.double(), s + bias.double().abs()
+    y = act64(v, act)
+    err = 1.13 * (k + 2) * 2.0**-23 * s
+    if act in ("gelu", "silu"):
+        err = err + 4e-6 * (1 + y.abs())
+    if residual is not None:
+        r = residual.double()
+        err = err + 2.0**-23 * (y.abs() + r.abs())
+        y = y + r
+    return y, err + 1.01 * ROUND[out_type] * y.abs() + STEP[out_type]
+
+
+def inputs(m, n, k, t, bias, residual, out_type, seed=0):
+    import torch
+
+    ty = _types()
+    g = torch.Generator(device="cuda").manual_seed(seed * 7919 + m * 31 + n * 17 + k)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    x, w = r(m, k).to(ty[t]), (r(n, k) * max(k, 1) ** -0.5).to(ty[t])
+    return (x, w, r(n).to(ty[t]) if bias else None, r(m, n).to(ty[out_type]) if residual else None,
+            torch.full((m, n), float("nan"), dtype=ty[out_type], device="cuda"))
+
+
+def check(got, y, bound):
+    d = (got.double() - y).abs()
+    over = ~(d <= bound)  # a NaN is over, too
+    assert not over.any(), (int(over.sum()), float(d[over].max()), over.nonzero()[:4].tolist())
+
+
+SIZES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (2, 7, 0), (1, 128, 64), (1, 513, 2048), (4, 64, 4096), (8, 96, 1000),
+         (16, 128, 256), (17, 129, 65), (31, 2, 130), (33, 1024, 512), (64, 200, 72), (65, 136, 776), (100, 77, 1003),
+         (128, 256, 128), (130, 300, 1000), (250, 512, 64), (257, 513, 129), (300, 640, 2056), (513, 1024, 776),
+         (1000, 2048, 96), (1, 4096, 4096), (129, 11008, 256), (2047, 385, 1024), (600, 4100, 520)]
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_sizes(cuda, m, n, k, t):
+    import torch
+
+    i = SIZES.index((m, n, k))
+    act, bias, residual = list(ACTS)[i % 4], i % 3 != 0, i % 2 == 1
+    x, w, b, r, y = inputs(m, n, k, t, bias, residual, t)
+    ref, bound = want(x, w, b, act, r, t)
+    torch.cuda.synchronize()
+    cuda.linear_dev(x, w, b, ACTS[act], r, y)
+    cuda.sync()
+    check(y, ref, bound)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 40, 4096), (20, 130, 264), (256, 256, 512), (700, 520, 1032), (65, 33, 45)])
+@pytest.mark.parametrize("act", list(ACTS))
+def test_f32_output_and_every_activation(cuda, m, n, k, act):
+    import torch
+
+    x, w, b, r, y = inputs(m, n, k, "bf16", True, True, "f32")
+    ref, bound = want(x, w, b, act, r, "f32")
+    torch.cuda.synchronize()
+    cuda.linear_dev(x, w, b, ACTS[act], r, y)
+    cuda.sync()
+    check(y, ref, bound)
+
+
+@pytest.mark.parametrize("m,n,k,pad", [(5, 30, 64, 8), (70, 130, 72, 8), (70, 130, 72, 1), (300, 264, 520, 24),
+                                       (300, 264, 520, 3), (1, 264, 512, 5)])
+def test_strided_rows_and_offset_bases(cuda, m, n, k, pad):
+    """Row strides that are and are not multiples of 16 bytes, bases one element into their buffers; what lies
+    between the rows stays."""
+    import torch
+
+    x, w, b, r, _ = inputs(m, n, k, "f16", True, True, "f16")
+
+    def strided(t, fill):
+        buf = torch.full((t.shape[0] * (t.shape[1] + pad) + pad,), fill, dtype=t.dtype, device="cuda")
+        v = buf[pad % 8:].as_strided((t.shape[0], t.shape[1]), (t.shape[1] + pad, 1))
+        v.copy_(t)
+        return buf, v
+
+    (_, xs), (_, ws), (_, rs) = strided(x, 3.0), strided(w, -5.0), strided(r, 9.0)
+    buf, ys = strided(torch.zeros(m, n, dtype=torch.float16, device="cuda"), 7.0)
+    ref, bound = want(x, w, b, "relu", r, "f16")
+    before = buf.clone()
+    torch.cuda.synchronize()
+    cuda.linear_dev(xs, ws, b, 1, rs, ys)
+    cuda.sync()
+    check(ys, ref, bound)
+    ys.zero_()
+    before_v = before[pad % 8:].as_strided((m, n), (n + pad, 1))
+    before_v.zero_()
+    assert torch.equal(buf, before)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 520), (48, 520, 256), (513, 264, 392), (40, 51, 77)])
+def test_residual_in_place(cuda, m, n, k):
+    import torch
+
+    x, w, b, r, _ = inputs(m, n, k, "bf16", True, True, "bf16")
+    ref, bound = want(x, w, b, "none", r, "bf16")
+    torch.cuda.synchronize()
+    cuda.linear_dev(x, w, b, 0, r, r)
+    cuda.sync()
+    check(r, ref, bound)
+
+
+@pytest.mark.parametrize("m,n,k", [(6, 140, 264), (70, 300, 520), (600, 520, 392), (9, 33, 51)])
+def test_infinities_and_nans_stay_in_their_rows(cuda, m, n, k):
+    import torch
+
+    x, w, b, r, y = inputs(m, n, k, "bf16", True, False, "bf16")
+    x[m // 2, k // 3] = float("nan")
+    x[m - 1, k - 1] = float("inf")
+    w[n - 1, 0] = float("nan")
+    ref, bound = want(x, w, b, "none", None, "bf16")
+    torch.cuda.synchronize()
+    cuda.linear_dev(x, w, b, 0, None, y)
+    cuda.sync()
+    bad = torch.zeros(m, n, dtype=torch.bool, device="cuda")
+    bad[m // 2] = True
+    bad[m - 1] = True
+    bad[:, n - 1] = True
+    assert torch.isnan(y[m // 2]).all() and torch.isnan(y[:, n - 1]).all()
+    assert not torch.isfinite(y[m - 1]).any()
+    check(y[~bad], ref[~bad], bound[~bad])
+
+
+def test_large_activations_saturate_like_the_formula(cuda):
+    """gelu and silu far from zero: 0 (or -0) on the left, the value itself on the right, no NaN from e^x."""
+    import torch
+
+    v = torch.tensor([-3e38, -1e4, -100.0, -90.0, -20.0, 0.0, 20.0, 90.0, 1e4, 3e38], device="cuda").bfloat16()
+    x, w = v[:, None].contiguous(), torch.ones(1, 1, dtype=torch.bfloat16, device="cuda")
+    for act in ("gelu", "silu"):
+        y = torch.empty(10, 1, dtype=torch.float32, device="cuda")
+        torch.cuda.synchronize()
+        cuda.linear_dev(x, w, None, ACTS[act], None, y)
+        cuda.sync()
+        got = y[:, 0].double()
+        left, right = v.double() < -80, v.double() > 15
+        assert (got[left].abs() < 1e-30).all()
+        assert ((got - v.double())[right].abs() <= 1e-6 * v.double()[right]).all()
+
+
+def test_zero_sizes_do_nothing(cuda):
+    import torch
+
+    e = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    cuda.linear_dev(e(0, 8), e(4, 8), None, 0, None, e(0, 4))
+    cuda.linear_dev(e(3, 8), e(0, 8), None, 0, None, e(3, 0))
+    cuda.sync()
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 260, 1000), (90, 520, 264), (400, 384, 520), (50, 70, 99)])
+def test_repeats_bit_for_bit_and_in_a_graph(cuda, m, n, k):
+    import torch
+
+    x, w, b, r, y = inputs(m, n, k, "f16", True, True, "f16")
+    torch.cuda.synchronize()
+    call = lambda: cuda.linear_dev(x, w, b, 2, r, y)  # noqa: E731
+    call()
+    cuda.sync()
+    first = y.clone()
+    g = cuda.capture(call)
+    for _ in range(3):
+        y.fill_(float("nan"))
+        torch.cuda.synchronize()
+        g.launch()
+        cuda.sync()
+        assert torch.equal(y, first)
+    g.close()
+
+
+def test_follows_the_backends_stream(cuda):
+    """Calls that feed one another on the backend's stream need no wait between them."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(64, 512, generator=g, device="cuda").bfloat16()
+    ws = [(torch.randn(512, 512, generator=g, device="cuda") * 512**-0.5).bfloat16() for _ in range(6)]
+    outs = [torch.empty_like(x) for _ in ws]
+    torch.cuda.synchronize()
+    cur = x
+    for w, o in zip(ws, outs):
+        cuda.linear_dev(cur, w, None, 0, None, o)
+        cur = o
+    cuda.sync()
+    cur = x
+    for w, o in zip(ws, outs):
+        ref, bound = want(cur, w, None, "none", None, "bf16")
+        check(o, ref, bound)
+        cur = o
+
+
+def test_refusals(cuda):
+    import torch
+
+    from tpt_infer_b200 import OpError
+    from tpt_infer_b200._capi import lib
+
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+
+    def refused(kind, *a):
+        with pytest.raises(OpError) as e:
+            cuda.linear_dev(*a)
+        assert e.value.kind == kind
+
+    refused("ShapeMismatch", z(2, 8), z(4, 9), None, 0, None, z(2, 4))
+    refused("ShapeMismatch", z(2, 8), z(4, 8), z(5), 0, None, z(2, 4))
+    refused("ShapeMismatch", z(2, 8), z(4, 8), None, 0, z(2, 5), z(2, 4))
+    refused("ShapeMismatch", z(2, 8), z(4, 8), None, 0, None, z(4, 2))
+    refused("ShapeMismatch", z(8, 2).t(), z(4, 8), None, 0, None, z(2, 4))
+    refused("ShapeMismatch", z(1, 8).expand(2, 8), z(4, 8), None, 0, None, z(2, 4))
+    refused("Unsupported", z(2, 8), z(4, 8, dt=torch.float16), None, 0, None, z(2, 4))
+    refused("Unsupported", z(2, 8, dt=torch.float32), z(4, 8, dt=torch.float32), None, 0, None,
+            z(2, 4, dt=torch.float32))
+    refused("Unsupported", z(2, 8), z(4, 8), None, 0, None, z(2, 4, dt=torch.float16))
+    refused("Invalid", z(2, 8), z(4, 8), None, 4, None, z(2, 4))
+    refused("Invalid", z(2, 8).cpu(), z(4, 8), None, 0, None, z(2, 4))
+    x, w, y = z(2, 8), z(4, 8), z(2, 4)
+    p = lambda t, off=0: C.c_void_p(t.data_ptr() + off)  # noqa: E731
+    bf = 2
+    assert lib.tpt_cuda_linear_dev(None, bf, p(x), 8, 2, 8, p(w), 8, 4, None, 0, None, 0, p(y), 4, bf) == 4
+    assert lib.tpt_cuda_linear_dev(cuda.ctx, bf, None, 8, 2, 8, p(w), 8, 4, None, 0, None, 0, p(y), 4, bf) == 4
+    assert lib.tpt_cuda_linear_dev(cuda.ctx, bf, p(x, 1), 8, 2, 8, p(w), 8, 4, None, 0, None, 0, p(y), 4, bf) == 4
+    assert lib.tpt_cuda_linear_dev(cuda.ctx, bf, p(x), 7, 2, 8, p(w), 8, 4, None, 0, None, 0, p(y), 4, bf) == 2
+    assert lib.tpt_cuda_linear_dev(cuda.ctx, 7, p(x), 8, 2, 8, p(w), 8, 4, None, 0, None, 0, p(y), 4, 7) == 3
+    assert lib.tpt_cuda_linear_dev(cuda.ctx, bf, p(x), 8, 1 << 31, 8, p(w), 8, 4, None, 0, None, 0, p(y), 4, bf) == 3
+    cuda.sync()

@@ -8,6 +8,7 @@ trait, plus the tpt-infer-quantize entry points) used by the tests and the
 benchmark. There is no CPU fallback: without the built library the import
 fails.
 """
-from .backend import (ACT_GELU, ACT_NONE, ACT_RELU, Conv2dOptions, CudaBackend, OpError, Weights)
+from .backend import (ACT_GELU, ACT_NONE, ACT_RELU, ACT_SILU, Conv2dOptions, CudaBackend, OpError, Weights)
 
-__all__ = ["CudaBackend", "Conv2dOptions", "OpError", "Weights", "ACT_NONE", "ACT_RELU", "ACT_GELU"]
+__all__ = ["CudaBackend", "Conv2dOptions", "OpError", "Weights", "ACT_NONE", "ACT_RELU", "ACT_GELU",
+           "ACT_SILU"]

@@ -104,6 +104,12 @@ SIGNATURES = {
     "tpt_cuda_plan_run_device": (C.c_int, [vp]),
     "tpt_cuda_plan_set_graph": (C.c_int, [vp, C.c_int]),
     "tpt_cuda_plan_run": (C.c_int, [vp, vp, vp, sz, vp, vp, sz]),
+    # 16-bit products and experts
+    "tpt_cuda_linear_dev": (C.c_int, [ctxp, C.c_int, vp, sz, sz, sz, vp, sz, sz, vp, C.c_int, vp, sz, vp, sz, C.c_int]),
+    "tpt_cuda_route_experts_dev": (C.c_int, [ctxp, vp, C.c_int, sz, sz, sz, C.c_int, vp, sz, sz, sz, sz, C.c_int,
+                                             C.c_float, vp, vp, vp]),
+    "tpt_cuda_experts_mlp_dev": (C.c_int, [ctxp, C.c_int, vp, sz, sz, sz, vp, vp, sz, vp, vp, sz, sz, C.c_int, C.c_int,
+                                           vp, sz, vp, sz]),
     # multi-GPU
     "tpt_cuda_comm_unique_id": (C.c_int, [vp, sz]),
     "tpt_cuda_comm_create": (C.c_int, [vp, vp, sz, C.c_int, C.c_int, C.POINTER(vp)]),
