@@ -263,7 +263,9 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
     size_t chunk = EXPERTS_WS_BYTES / per_token;
     if (chunk < 1) chunk = 1;
     if (chunk > tokens) chunk = tokens;
-    const int tile_rows = 64;
+    // tokens per tile: what an expert gets on average, up to the pair kernel's 256
+    const size_t mean = (tokens * top_k + experts - 1) / experts;
+    const int tile_rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
     for (size_t t0 = 0; t0 < tokens; t0 += chunk) {
         const size_t tn = tokens - t0 < chunk ? tokens - t0 : chunk;
         const size_t pairs = tn * top_k;
@@ -299,6 +301,7 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
         g.tiles = tiles;
         g.n_tiles = n_tiles;
         g.max_tiles = (int)max_tiles;
+        g.tile_rows = tile_rows;
         g.act = act;
         g.gated = gated;
         g.y = ctx->ws + o_h;
@@ -319,6 +322,7 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
         o.tiles = tiles;
         o.n_tiles = n_tiles;
         o.max_tiles = (int)max_tiles;
+        o.tile_rows = tile_rows;
         o.y = ctx->ws + o_p;
         o.ldy = d;
         o.y_f32 = true;

@@ -17,10 +17,13 @@ __global__ void __launch_bounds__(256) k_gemm16_simple(Gemm16 g) {
     __shared__ float xs[SK][SB + 4], ws[SK][SB + 4], us[GATED ? SK : 1][SB + 4];
     int row0, rows, expert = 0;
     if (g.tiles) {
-        if ((int)blockIdx.y >= *g.n_tiles) return;
-        const Tile16 t = g.tiles[blockIdx.y];
-        row0 = t.row0;
-        rows = t.rows;
+        const int sub = (g.tile_rows + SB - 1) / SB;
+        const int ti = blockIdx.y / sub, off = (blockIdx.y - ti * sub) * SB;
+        if (ti >= *g.n_tiles) return;
+        const Tile16 t = g.tiles[ti];
+        if (off >= t.rows) return;
+        row0 = t.row0 + off;
+        rows = min(SB, t.rows - off);
         expert = t.expert;
     } else {
         row0 = blockIdx.y * SB;
@@ -81,7 +84,7 @@ __global__ void __launch_bounds__(256) k_gemm16_simple(Gemm16 g) {
 
 template <typename T>
 int launch_simple(tpt_cuda_ctx *ctx, const Gemm16 &g) {
-    const dim3 grid((g.n + SB - 1) / SB, g.tiles ? g.max_tiles : (g.rows + SB - 1) / SB);
+    const dim3 grid((g.n + SB - 1) / SB, g.tiles ? g.max_tiles * ((g.tile_rows + SB - 1) / SB) : (g.rows + SB - 1) / SB);
     if (g.gated)
         launch_pdl(k_gemm16_simple<T, T, true>, grid, 256, 0, ctx->stream, g);
     else if (g.y_f32)
@@ -94,6 +97,7 @@ int launch_simple(tpt_cuda_ctx *ctx, const Gemm16 &g) {
 }  // namespace
 
 int launch_gemm16(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
+    if (gemm16_tc_ok(g)) return launch_gemm16_tc(ctx, dtype, g);
     return dtype == TPT_DT_BF16 ? launch_simple<__nv_bfloat16>(ctx, g) : launch_simple<__half>(ctx, g);
 }
 

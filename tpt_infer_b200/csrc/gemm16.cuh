@@ -30,6 +30,7 @@ struct Gemm16 {
     const Tile16 *tiles = nullptr;
     const int *n_tiles = nullptr;
     int max_tiles = 0;  // grouped: no schedule has more
+    int tile_rows = 0;  // grouped: no tile has more rows
     const void *bias = nullptr;
     int act = 0;
     bool gated = false;
@@ -42,6 +43,9 @@ struct Gemm16 {
 
 // device enqueue; dtype TPT_DT_BF16 or TPT_DT_F16
 int launch_gemm16(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g);
+// the tensor-core kernels: whether TMA can read the operands, and the launch
+bool gemm16_tc_ok(const Gemm16 &g);
+int launch_gemm16_tc(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g);
 
 #ifdef __CUDACC__
 

@@ -1,0 +1,832 @@
+// gemm16_tc.cu -- the 16-bit products on the tensor cores (tcgen05.mma
+// kind::f16, f32 accumulators in tensor memory).
+//
+// The weights are the MMA's M side and the tokens its N side: an expert's
+// weights stream through 128-row tiles whatever its number of tokens, and the
+// number of columns follows the tokens in steps of 16 or 32, so a short list
+// of tokens costs no padded rows of 128. A tensor-memory lane is an output
+// feature and its columns are tokens: the bias is one register, and a warp's
+// store of one column is 32 consecutive features of one row.
+//
+//   k_gemm16_pair   256 weight rows x up to 256 tokens per pair of SMs
+//                   (cta_group::2), persistent, for work bound by the MMA
+//   k_gemm16_split  128 weight rows x up to 128 tokens per SM, k split over a
+//                   cluster, for work bound by the weights' stream
+//
+// Gated layers: each 32-lane quarter holds 16 gate rows and the 16 up rows of
+// the same features (one TMA box over the two halves of W), so the two meet
+// by one exchange between lanes l and l + 16.
+//
+// Every wait is bounded; a wait that runs out raises the CTA's abort and the
+// context's timeout word, the roles leave, copies and MMAs in flight are
+// drained (bounded), tensor memory is freed and the kernel returns.
+#include "gemm16.cuh"
+
+namespace tpt {
+namespace {
+using namespace tc;
+
+constexpr int BK = 64;           // k values per stage: one 128-byte swizzled row
+constexpr int ROW_BYTES = 128;
+constexpr int W_ROWS = 128;      // weight rows of one CTA's tile
+constexpr int W_BYTES = W_ROWS * ROW_BYTES;
+
+struct Args {
+    int rows, n, k;
+    int ftiles;                  // feature tiles
+    int tile_n;                  // dense: tokens per tile
+    int box_rows;                // X's box (no gather)
+    int group;                   // dense: token tiles that share a sweep over the features
+    uint32_t fmt;                // 0 f16, 1 bf16
+    const int *row_token;
+    const Tile16 *tiles;
+    const int *n_tiles;
+    const void *bias;
+    int act;
+    const void *residual;
+    size_t ldr;
+    void *y;
+    size_t ldy;
+    unsigned *gflags;
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+        "[%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, int y, int z,
+                                            int u) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, "
+        "%6}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u)
+        : "memory");
+}
+// four rows of a 2-D map (box one row high)
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, const int (&r)[4]) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+        "%4, %5, %6, %7}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3])
+        : "memory");
+}
+// The same loads of an SM pair: the bytes count on the barrier at `bar`, the
+// leader CTA's (a shared::cluster address).
+__device__ __forceinline__ void tma_load_2d_p(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+        "{%3, %4}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_p(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+        "{%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d_p(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, int y, int z,
+                                              int u) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+        "{%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y), "r"(z),
+        "r"(u)
+        : "memory");
+}
+__device__ __forceinline__ void tma_gather4_p(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x,
+                                              const int (&r)[4]) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+        : "memory");
+}
+
+template <int GROUP>
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+    if constexpr (GROUP == 2)
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+// f32 accumulator, both operands K-major of type fmt, M x N
+__device__ __forceinline__ uint32_t idesc_f16(uint32_t fmt, uint32_t m, uint32_t n) {
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+__device__ __forceinline__ void commit_both(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+// C columns (tokens col0 .. col0 + C - 1 of the tile) of this thread's lane.
+// Ungated: lane l of the warp is feature f0 + l. Gated: lanes l and l + 16 are
+// the gate and the up product of feature f0 + l; each of them finishes half of
+// the columns.
+template <typename T, typename TY, bool GATED, int C>
+__device__ __forceinline__ void epilogue16(const Args &a, float (&v)[C], int f0, size_t row0, int col0, int rows,
+                                           int lane) {
+    if constexpr (GATED) {
+        const bool hi = lane >= 16;
+        const int f = f0 + (lane & 15);
+        float h[C / 2];
+#pragma unroll
+        for (int i = 0; i < C / 2; i++) {
+            const float got = __shfl_xor_sync(0xffffffffu, hi ? v[i] : v[C / 2 + i], 16);
+            const float g = hi ? got : v[i], u = hi ? v[C / 2 + i] : got;
+            h[i] = act16(g, a.act) * u;
+        }
+        const int c0 = col0 + (hi ? C / 2 : 0);
+        TY *y = static_cast<TY *>(a.y) + (row0 + c0) * a.ldy + f;
+        if (f < a.n) {
+#pragma unroll
+            for (int i = 0; i < C / 2; i++)
+                if (c0 + i < rows) y[(size_t)i * a.ldy] = from_f32<TY>(h[i]);
+        }
+    } else {
+        const int f = f0 + lane;
+        if (f >= a.n) return;
+        const float b = a.bias ? to_f32(static_cast<const T *>(a.bias)[f]) : 0.0f;
+        TY *y = static_cast<TY *>(a.y) + (row0 + col0) * a.ldy + f;
+        if (a.residual) {
+            const TY *r = static_cast<const TY *>(a.residual) + (row0 + col0) * a.ldr + f;
+            float rv[C];
+#pragma unroll
+            for (int i = 0; i < C; i++) rv[i] = col0 + i < rows ? to_f32(r[(size_t)i * a.ldr]) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < C; i++) v[i] = act16(v[i] + b, a.act) + rv[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < C; i++) v[i] = act16(v[i] + b, a.act);
+        }
+#pragma unroll
+        for (int i = 0; i < C; i++)
+            if (col0 + i < rows) y[(size_t)i * a.ldy] = from_f32<TY>(v[i]);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The SM-pair kernel. Barriers as in the pair's INT8 kernel:
+//   full[s]   (leader)  both CTAs' bytes of stage s
+//   empty[s]  (each)    the leader's MMAs have read stage s
+//   tfull[b]  (each)    accumulator b is complete
+//   tempty[b] (leader)  both CTAs' epilogue warps have read accumulator b
+// ---------------------------------------------------------------------------
+constexpr int P_STAGES = 6;
+constexpr int P_STAGE_BYTES = 2 * W_BYTES;  // 128 weight rows + up to 128 token rows
+constexpr int P_EPI_WARPS = 8;
+constexpr int P_THREADS = (2 + P_EPI_WARPS) * 32;
+constexpr int P_SMEM = P_STAGES * P_STAGE_BYTES + (2 * P_STAGES + 5) * 8 + 1024;
+
+struct TileAt {
+    int expert, row0, rows, cols, ft;
+};
+// Tile t of the product. Dense: sweeps of `group` token tiles over all the
+// features, so that the tiles in flight share both operands in L2.
+__device__ __forceinline__ TileAt tile_at(const Args &a, int t) {
+    TileAt r;
+    if (a.tiles) {
+        const int i = t / a.ftiles;
+        r.ft = t - i * a.ftiles;
+        const int4 q = __ldcg(reinterpret_cast<const int4 *>(a.tiles) + i);
+        r.expert = q.x;
+        r.row0 = q.y;
+        r.rows = q.z;
+        r.cols = (q.z + 31) & ~31;
+    } else {
+        const int ttiles = (a.rows + a.tile_n - 1) / a.tile_n;
+        const int sweep = a.group * a.ftiles;
+        const int s = t / sweep, in = t - s * sweep;
+        const int wide = min(a.group, ttiles - s * a.group);
+        r.ft = in / wide;
+        const int tt = s * a.group + in - r.ft * wide;
+        r.expert = 0;
+        r.row0 = tt * a.tile_n;
+        r.rows = min(a.tile_n, a.rows - r.row0);
+        r.cols = a.tile_n;
+    }
+    return r;
+}
+
+template <typename T, typename TY, bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
+    k_gemm16_pair(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                  const __grid_constant__ Args a) {
+    constexpr int S = P_STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int abort_flag;
+    __shared__ uint32_t tmem_slot;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t bars = ring + S * P_STAGE_BYTES;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
+    auto tfull_bar = [&](int b) { return bars + 8u * (2 * S + b); };
+    auto tempty_bar = [&](int b) { return bars + 8u * (2 * S + 2 + b); };
+    const uint32_t drain_bar = bars + 8u * (2 * S + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const bool leader = rank == 0;
+    const int cluster = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
+    const int kblocks = (a.k + BK - 1) / BK;
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < S; s++) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(tfull_bar(b), 1);
+            mbar_init(tempty_bar(b), 2 * P_EPI_WARPS);
+        }
+        mbar_init(drain_bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmW)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                     "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t tmem = tmem_slot;
+    volatile int *abort_p = &abort_flag;
+    const int ntiles = a.tiles ? __ldcg(a.n_tiles) * a.ftiles : ((a.rows + a.tile_n - 1) / a.tile_n) * a.ftiles;
+
+    if (warp == 0) {
+        // ---------------- producer: lane 0 the boxes, every lane four gathered rows ----------------
+        int stage = 0;
+        uint32_t phase = 0;
+        int issued = 0;
+        bool ok = true;
+        for (int t = cluster; t < ntiles && ok; t += nclusters) {
+            const TileAt tl = tile_at(a, t);
+            const int half = tl.cols >> 1;
+            const uint32_t bytes = 2u * (W_BYTES + half * ROW_BYTES);
+            const int xrow = tl.row0 + (int)rank * half;
+            int r4[4];
+            if (a.row_token) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {  // past the tile's rows: its first row, into columns that nothing reads
+                    const int c = (int)rank * half + lane * 4 + i;
+                    r4[i] = __ldcg(a.row_token + tl.row0 + (c < tl.rows ? c : 0));
+                }
+            }
+            for (int kb = 0; kb < kblocks; kb++) {
+                if (lane == 0) ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_p, a.gflags, true);
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
+                const uint32_t w_dst = ring + stage * P_STAGE_BYTES, x_dst = w_dst + W_BYTES;
+                const uint32_t fb = map_to_rank(full_bar(stage), 0);
+                if (lane == 0) {
+                    if (leader) mbar_arrive_expect_tx(full_bar(stage), bytes);
+                    if (GATED) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+                            tma_load_4d_p(w_dst + q * 4096, &tmW, fb, kb * BK, tl.ft * 128 + (int)rank * 64 + q * 16,
+                                          0, tl.expert);
+                    } else {
+                        tma_load_3d_p(w_dst, &tmW, fb, kb * BK, tl.ft * 256 + (int)rank * 128, tl.expert);
+                    }
+                    if (!a.row_token)
+                        for (int r = 0; r < half; r += a.box_rows)
+                            tma_load_2d_p(x_dst + r * ROW_BYTES, &tmX, fb, kb * BK, xrow + r);
+                }
+                __syncwarp();
+                if (a.row_token && lane * 4 < half) tma_gather4_p(x_dst + lane * 4 * ROW_BYTES, &tmX, fb, kb * BK, r4);
+                issued++;
+                if (++stage == S) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        // an aborting pair leaves no copy in flight behind it: the leader waits
+        // (bounded) for the stages it announced and did not see consumed
+        if (!ok && leader && lane == 0) {
+            const int n = issued < S ? issued : S;
+            for (int i = 0; i < n; i++) {
+                if (--stage < 0) {
+                    stage = S - 1;
+                    phase ^= 1u;
+                }
+                mbar_wait(full_bar(stage), phase, abort_p, a.gflags, false);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            // ---------------- MMA issuer ----------------
+            int stage = 0;
+            uint32_t phase = 0;
+            int acc = 0;
+            uint32_t acc_phase = 0;
+            bool ok = true;
+            for (int t = cluster; t < ntiles && ok; t += nclusters) {
+                const uint32_t idesc = idesc_f16(a.fmt, 256, tile_at(a, t).cols);
+                if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_p, a.gflags, true)) break;
+                tc_fence_after();
+                const uint32_t d_tmem = tmem + (uint32_t)(acc * 256);
+                for (int kb = 0; kb < kblocks; kb++) {
+                    if (!mbar_wait(full_bar(stage), phase, abort_p, a.gflags, true)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t w_addr = ring + stage * P_STAGE_BYTES, x_addr = w_addr + W_BYTES;
+#pragma unroll
+                    for (int kk = 0; kk < BK / 16; kk++)
+                        mma_f16<2>(d_tmem, sw128_desc(w_addr + 32 * kk), sw128_desc(x_addr + 32 * kk), idesc,
+                                   (kb | kk) != 0 ? 1u : 0u);
+                    commit_both(empty_bar(stage));
+                    if (++stage == S) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                commit_both(tfull_bar(acc));
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
+            }
+            // drain: every MMA issued completes before tensor memory is freed
+            asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain_bar)
+                         : "memory");
+            mbar_wait(drain_bar, 0, abort_p, a.gflags, false);
+        }
+    } else {
+        // ---------------- epilogue: two warps per lane quarter, alternate 32-column chunks ----------------
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t tempty_leader0 = map_to_rank(tempty_bar(0), 0);
+        const uint32_t tempty_leader1 = map_to_rank(tempty_bar(1), 0);
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        for (int t = cluster; t < ntiles; t += nclusters) {
+            const TileAt tl = tile_at(a, t);
+            int okw = 0;
+            if (lane == 0) okw = mbar_wait(tfull_bar(acc), acc_phase, abort_p, a.gflags, true) ? 1 : 0;
+            okw = __shfl_sync(0xffffffffu, okw, 0);
+            if (!okw) break;
+            tc_fence_after();
+            const int f0 = GATED ? tl.ft * 128 + (int)rank * 64 + q * 16 : tl.ft * 256 + (int)rank * 128 + q * 32;
+            const uint32_t t_base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 256);
+#pragma unroll 1
+            for (int c = half * 32; c < tl.rows; c += 64) {
+                float v[32];
+                tmem_ld32(t_base + (uint32_t)c, reinterpret_cast<uint32_t(&)[32]>(v));
+                tmem_wait_ld();
+                epilogue16<T, TY, GATED, 32>(a, v, f0, (size_t)tl.row0, c, tl.rows, lane);
+                __syncwarp();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(acc == 0 ? tempty_leader0 : tempty_leader1);
+            if (++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1u;
+            }
+        }
+        __syncwarp();
+    }
+    // both CTAs stay until neither needs the other's memory or barriers
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The split kernel: one tile of 128 weight rows x NT tokens per cluster of KS
+// CTAs, each on its share of k. The CTAs' partial sums meet in distributed
+// shared memory: CTA r adds the columns [r NT / KS, (r + 1) NT / KS) of all of
+// them in rank order (a fixed order) and finishes those. Two CTAs fit on an
+// SM, so one streams while the other starts or finishes.
+// ---------------------------------------------------------------------------
+constexpr int S_THREADS = 6 * 32;
+
+template <int NT>
+struct SplitCfg {
+    static constexpr int STAGE_BYTES = W_BYTES + NT * ROW_BYTES;
+    static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 3;
+    static constexpr int TMEM_COLS = NT < 32 ? 32 : NT;
+    static constexpr int SMEM = STAGES * STAGE_BYTES + (2 * STAGES + 1) * 8 + 1024;
+    static_assert(STAGES * STAGE_BYTES >= NT * W_ROWS * 4, "the partial sums reuse the ring");
+    static_assert(2 * (SMEM + 1024) <= 233472, "two CTAs per SM");
+};
+
+template <typename T, typename TY, bool GATED, int NT, int KS>
+__global__ void __launch_bounds__(S_THREADS, 2)
+    k_gemm16_split(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                   const __grid_constant__ Args a) {
+    using Cfg = SplitCfg<NT>;
+    constexpr int S = Cfg::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int abort_flag;
+    __shared__ uint32_t tmem_slot;
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t ring = (raw + 1023u) & ~1023u;
+    const uint32_t bars = ring + S * Cfg::STAGE_BYTES;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
+    const uint32_t done_bar = bars + 8u * (2 * S);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = KS > 1 ? (int)cluster_rank() : 0;
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < S; s++) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        mbar_init(done_bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmW)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                     "r"((uint32_t)Cfg::TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t tmem = tmem_slot;
+    volatile int *abort_p = &abort_flag;
+
+    const int t = (int)blockIdx.x / KS;
+    const int ti = t / a.ftiles, ft = t - ti * a.ftiles;
+    int expert = 0, row0, rows;
+    if (a.tiles) {
+        const bool in = ti < __ldcg(a.n_tiles);  // the grid has room for the longest schedule
+        const int4 q = in ? __ldcg(reinterpret_cast<const int4 *>(a.tiles) + ti) : make_int4(0, 0, 0, 0);
+        expert = q.x;
+        row0 = q.y;
+        rows = q.z;
+    } else {
+        row0 = ti * NT;
+        rows = min(NT, a.rows - row0);
+    }
+    const int all_kb = (a.k + BK - 1) / BK;
+    const int kb0 = all_kb * rank / KS, kb1 = all_kb * (rank + 1) / KS;  // KS <= all_kb
+    if (rows > 0) {  // the same for every CTA of the cluster
+        if (warp == 0) {
+            // ---------------- producer ----------------
+            int r4[4];
+            if (a.row_token) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {  // past the tile's rows: its first row, into columns that nothing reads
+                    const int c = lane * 4 + i;
+                    r4[i] = __ldcg(a.row_token + row0 + (c < rows ? c : 0));
+                }
+            }
+            bool ok = true;
+            int stage = 0, issued = 0;
+            uint32_t phase = 0;
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (lane == 0) ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_p, a.gflags, true);
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
+                const uint32_t w_dst = ring + stage * Cfg::STAGE_BYTES, x_dst = w_dst + W_BYTES;
+                const uint32_t fb = full_bar(stage);
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(fb, Cfg::STAGE_BYTES);
+                    if (GATED) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+                            tma_load_4d(w_dst + q * 4096, &tmW, fb, kb * BK, ft * 64 + q * 16, 0, expert);
+                    } else {
+                        tma_load_3d(w_dst, &tmW, fb, kb * BK, ft * 128, expert);
+                    }
+                    if (!a.row_token) tma_load_2d(x_dst, &tmX, fb, kb * BK, row0);
+                }
+                __syncwarp();
+                if (a.row_token && lane * 4 < NT) tma_gather4(x_dst + lane * 4 * ROW_BYTES, &tmX, fb, kb * BK, r4);
+                issued++;
+                if (++stage == S) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (!ok && lane == 0) {  // aborting: no copy stays in flight
+                const int n = issued < S ? issued : S;
+                for (int i = 0; i < n; i++) {
+                    if (--stage < 0) {
+                        stage = S - 1;
+                        phase ^= 1u;
+                    }
+                    mbar_wait(full_bar(stage), phase, abort_p, a.gflags, false);
+                }
+            }
+        } else if (warp == 1) {
+            if (lane == 0) {
+                // ---------------- MMA issuer ----------------
+                const uint32_t idesc = idesc_f16(a.fmt, 128, NT);
+                int stage = 0;
+                uint32_t phase = 0;
+                for (int kb = kb0; kb < kb1; kb++) {
+                    if (!mbar_wait(full_bar(stage), phase, abort_p, a.gflags, true)) break;
+                    tc_fence_after();
+                    const uint32_t w_addr = ring + stage * Cfg::STAGE_BYTES, x_addr = w_addr + W_BYTES;
+#pragma unroll
+                    for (int kk = 0; kk < BK / 16; kk++)
+                        mma_f16<1>(tmem, sw128_desc(w_addr + 32 * kk), sw128_desc(x_addr + 32 * kk), idesc,
+                                   kb > kb0 || kk > 0 ? 1u : 0u);
+                    tc_commit(empty_bar(stage));
+                    if (++stage == S) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                tc_commit(done_bar);
+                mbar_wait(done_bar, 0, abort_p, a.gflags, false);
+            }
+        }
+        // ---------------- epilogue (warps 2 to 5) ----------------
+        int go = 0;
+        if (warp >= 2) {
+            if (lane == 0) go = mbar_wait(done_bar, 0, abort_p, a.gflags, true) ? 1 : 0;
+            go = __shfl_sync(0xffffffffu, go, 0);
+            tc_fence_after();
+        }
+        __syncwarp();
+        const int q = warp & 3;
+        const int f0 = GATED ? ft * 64 + q * 16 : ft * 128 + q * 32;
+        const uint32_t t_base = tmem + ((uint32_t)(q * 32) << 16);
+        if constexpr (KS == 1) {
+            if (go) {
+                constexpr int C = NT < 32 ? NT : 32;
+#pragma unroll 1
+                for (int c = 0; c < NT && c < rows; c += C) {
+                    float v[C];
+                    if constexpr (C == 32)
+                        tmem_ld32(t_base + (uint32_t)c, reinterpret_cast<uint32_t(&)[32]>(v));
+                    else
+                        tmem_ld16(t_base + (uint32_t)c, reinterpret_cast<uint32_t *>(v));
+                    tmem_wait_ld();
+                    epilogue16<T, TY, GATED, C>(a, v, f0, (size_t)row0, c, rows, lane);
+                    __syncwarp();
+                }
+            }
+        } else {
+            constexpr int CW = NT / KS;  // columns that each CTA finishes
+            cluster_sync();              // every CTA's MMAs and copies are done: the rings are free
+            if (warp >= 2) {
+#pragma unroll 1
+                for (int c = 0; c < NT; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(t_base + (uint32_t)c, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int o = (c + i) / CW, oc = (c + i) % CW;
+                        const uint32_t dst = map_to_rank(ring, (uint32_t)o) +
+                                             (uint32_t)(((rank * CW + oc) * W_ROWS + q * 32 + lane) * 4);
+                        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(dst), "r"(v[i]) : "memory");
+                    }
+                }
+            }
+            __syncwarp();
+            cluster_sync();
+            const int c0 = rank * CW;
+            if (go && c0 < rows) {
+                const float *part = reinterpret_cast<const float *>(smem_raw + (ring - raw)) + q * 32 + lane;
+                constexpr int C = CW < 16 ? CW : 16;
+#pragma unroll 1
+                for (int c = 0; c < CW; c += C) {
+                    float v[C];
+#pragma unroll
+                    for (int i = 0; i < C; i++) {
+                        v[i] = part[(c + i) * W_ROWS];
+#pragma unroll
+                        for (int s = 1; s < KS; s++) v[i] += part[(s * CW + c + i) * W_ROWS];
+                    }
+                    epilogue16<T, TY, GATED, C>(a, v, f0, (size_t)row0, c0 + c, rows, lane);
+                    __syncwarp();
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)Cfg::TMEM_COLS)
+                     : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+// Tensor map of 16-bit elements with 64-wide, 128B-swizzled boxes; dims and
+// strides from the innermost out, strides of the outer dims in elements.
+bool make_map(CUtensorMap *tm, int dtype, const void *base, int rank, const size_t *dims, const size_t *strides,
+              const unsigned *box) {
+    auto fn = encode_fn();
+    if (!fn || ((uintptr_t)base & 15)) return false;
+    cuuint64_t d[4], s[3];
+    cuuint32_t b[4], e[4] = {1, 1, 1, 1};
+    for (int i = 0; i < rank; i++) {
+        d[i] = dims[i];
+        b[i] = box[i];
+        if (i) {
+            s[i - 1] = strides[i - 1] * 2;
+            if (s[i - 1] & 15) return false;
+        }
+    }
+    return fn(tm, dtype == TPT_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+              (cuuint32_t)rank, const_cast<void *>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool weight_map(CUtensorMap *tm, int dtype, const Gemm16 &g) {
+    const size_t ldw = g.n > 1 || g.gated ? g.ldw : (size_t)(g.k + 7) / 8 * 8;
+    const size_t we = g.experts > 1 ? g.w_expert : (size_t)(g.gated ? 2 : 1) * g.n * ldw;
+    if (g.gated) {
+        const size_t dims[4] = {(size_t)g.k, (size_t)g.n, 2, (size_t)g.experts}, st[3] = {ldw, (size_t)g.n * ldw, we};
+        const unsigned box[4] = {BK, 16, 2, 1};
+        return make_map(tm, dtype, g.w, 4, dims, st, box);
+    }
+    const size_t dims[3] = {(size_t)g.k, (size_t)g.n, (size_t)g.experts}, st[2] = {ldw, we};
+    const unsigned box[3] = {BK, W_ROWS, 1};
+    return make_map(tm, dtype, g.w, 3, dims, st, box);
+}
+bool token_map(CUtensorMap *tm, int dtype, const Gemm16 &g, unsigned box_rows) {
+    const size_t ldx = g.x_rows > 1 ? g.ldx : (size_t)(g.k + 7) / 8 * 8;
+    const size_t dims[2] = {(size_t)g.k, (size_t)g.x_rows}, st[1] = {ldx};
+    const unsigned box[2] = {BK, g.row_token ? 1u : box_rows};
+    return make_map(tm, dtype, g.x, 2, dims, st, box);
+}
+
+Args make_args(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
+    Args a = {};
+    a.rows = g.rows;
+    a.n = g.n;
+    a.k = g.k;
+    a.fmt = dtype == TPT_DT_BF16 ? 1 : 0;
+    a.row_token = g.row_token;
+    a.tiles = g.tiles;
+    a.n_tiles = g.n_tiles;
+    a.bias = g.bias;
+    a.act = g.act;
+    a.residual = g.residual;
+    a.ldr = g.ldr;
+    a.y = g.y;
+    a.ldy = g.ldy;
+    a.gflags = ctx->d_flags;
+    return a;
+}
+
+template <typename T, typename TY, bool GATED>
+int launch_pair(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g, int tile_n) {
+    auto kern = k_gemm16_pair<T, TY, GATED>;
+    static int cached[64] = {};  // pairs of SMs that hold a cluster at the same time
+    const int dev = ctx->device & 63;
+    if (!cached[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM);
+        if (e != cudaSuccess) return cuda_fail(ctx, e, "gemm16_pair smem attribute");
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * (ctx->sm_count / 2), 1, 1);
+        cfg.blockDim = dim3(P_THREADS, 1, 1);
+        cfg.dynamicSmemBytes = P_SMEM;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = 2;
+        at[0].val.clusterDim.y = 1;
+        at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+            cudaGetLastError();
+            n = ctx->sm_count / 2;
+        }
+        cached[dev] = n;
+    }
+    const int pairs = cached[dev];
+    Args a = make_args(ctx, dtype, g);
+    a.ftiles = (g.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
+    a.tile_n = tile_n;
+    a.box_rows = g.tiles ? 16 : tile_n / 2;
+    a.group = 8;
+    CUtensorMap tw, tx;
+    if (!weight_map(&tw, dtype, g) || !token_map(&tx, dtype, g, (unsigned)a.box_rows))
+        return cuda_fail(ctx, cudaErrorInvalidValue, "gemm16_pair tensor map");
+    const long long tiles = (g.tiles ? (long long)g.max_tiles : ((long long)g.rows + tile_n - 1) / tile_n) * a.ftiles;
+    if (tiles > 0x7fffffffLL) return TPT_UNSUPPORTED;
+    const int clusters = tiles < pairs ? (int)tiles : pairs;
+    launch_pdl(kern, 2 * clusters, P_THREADS, P_SMEM, ctx->stream, tw, tx, a);
+    return after_launch(ctx, "gemm16_pair");
+}
+
+template <typename T, typename TY, bool GATED, int NT, int KS>
+int launch_split(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
+    using Cfg = SplitCfg<NT>;
+    auto kern = k_gemm16_split<T, TY, GATED, NT, KS>;
+    static bool done[64] = {};
+    const int dev = ctx->device & 63;
+    if (!done[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+        // the largest carveout, or only one CTA would fit per SM
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        if (e != cudaSuccess) return cuda_fail(ctx, e, "gemm16_split smem attribute");
+        done[dev] = true;
+    }
+    Args a = make_args(ctx, dtype, g);
+    a.ftiles = (g.n + (GATED ? 63 : 127)) / (GATED ? 64 : 128);
+    CUtensorMap tw, tx;
+    if (!weight_map(&tw, dtype, g) || !token_map(&tx, dtype, g, NT))
+        return cuda_fail(ctx, cudaErrorInvalidValue, "gemm16_split tensor map");
+    const long long tiles = (g.tiles ? (long long)g.max_tiles : ((long long)g.rows + NT - 1) / NT) * a.ftiles;
+    if (tiles * KS > 0x7fffffffLL) return TPT_UNSUPPORTED;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * KS));
+    cfg.blockDim = dim3(S_THREADS);
+    cfg.dynamicSmemBytes = Cfg::SMEM;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = KS;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = KS > 1 ? 2 : 1;
+    (void)cudaLaunchKernelEx(&cfg, kern, tw, tx, a);
+    return after_launch(ctx, "gemm16_split");
+}
+
+template <typename T, typename TY, bool GATED, int NT>
+int launch_split_k(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g, int ks) {
+    if (ks >= 8) return launch_split<T, TY, GATED, NT, 8>(ctx, dtype, g);
+    if (ks >= 4) return launch_split<T, TY, GATED, NT, 4>(ctx, dtype, g);
+    if (ks >= 2) return launch_split<T, TY, GATED, NT, 2>(ctx, dtype, g);
+    return launch_split<T, TY, GATED, NT, 1>(ctx, dtype, g);
+}
+
+template <typename T, typename TY, bool GATED>
+int launch_tc(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
+    const int fw = GATED ? 64 : 128;  // features of a split tile
+    const long long ft = (g.n + fw - 1) / fw;
+    const int kb = (g.k + BK - 1) / BK;
+    if (g.tiles ? g.tile_rows > 128 : g.rows > 256) return launch_pair<T, TY, GATED>(ctx, dtype, g, 256);
+    const int nt = g.tiles ? g.tile_rows : g.rows <= 16 ? 16 : g.rows <= 32 ? 32 : g.rows <= 64 ? 64 : 128;
+    const long long tiles = (g.tiles ? (long long)g.max_tiles : ((long long)g.rows + nt - 1) / nt) * ft;
+    int ks = 1;
+    while (ks < 8 && tiles * ks * 2 <= 2LL * ctx->sm_count && kb / (ks * 2) >= 4) ks *= 2;
+    if (nt == 16) return launch_split_k<T, TY, GATED, 16>(ctx, dtype, g, ks);
+    if (nt == 32) return launch_split_k<T, TY, GATED, 32>(ctx, dtype, g, ks);
+    if (nt == 64) return launch_split_k<T, TY, GATED, 64>(ctx, dtype, g, ks);
+    return launch_split_k<T, TY, GATED, 128>(ctx, dtype, g, ks);
+}
+
+template <typename T>
+int launch_typed(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
+    if (g.gated) return launch_tc<T, T, true>(ctx, dtype, g);
+    if (g.y_f32) return launch_tc<T, float, false>(ctx, dtype, g);
+    return launch_tc<T, T, false>(ctx, dtype, g);
+}
+
+}  // namespace
+
+bool gemm16_tc_ok(const Gemm16 &g) {
+    auto al = [](const void *p) { return ((uintptr_t)p & 15) == 0; };
+    return g.k > 0 && al(g.x) && al(g.w) && (g.x_rows <= 1 || g.ldx % 8 == 0) &&
+           ((g.n <= 1 && !g.gated) || g.ldw % 8 == 0) &&
+           (!g.gated || ((size_t)g.n * g.ldw) % 8 == 0) && (g.experts <= 1 || g.w_expert % 8 == 0);
+}
+
+int launch_gemm16_tc(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
+    return dtype == TPT_DT_BF16 ? launch_typed<__nv_bfloat16>(ctx, dtype, g) : launch_typed<__half>(ctx, dtype, g);
+}
+
+}  // namespace tpt
