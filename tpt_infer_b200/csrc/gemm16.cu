@@ -68,13 +68,17 @@ __global__ void __launch_bounds__(256) k_gemm16_simple(Gemm16 g) {
     for (int i = 0; i < 4; i++) {
         const int r = ty * 4 + i;
         if (r >= rows) continue;
+        if (g.bias) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (f0 + tx * 4 + j < g.n) acc[i][j] += to_f32(static_cast<const T *>(g.bias)[f0 + tx * 4 + j]);
+        }
+        act16(acc[i], g.act);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int f = f0 + tx * 4 + j;
             if (f >= g.n) continue;
             float v = acc[i][j];
-            if (g.bias) v += to_f32(static_cast<const T *>(g.bias)[f]);
-            v = act16(v, g.act);
             if (GATED) v *= up[i][j];
             if (g.residual) v += to_f32(static_cast<const TY *>(g.residual)[(size_t)(row0 + r) * g.ldr + f]);
             static_cast<TY *>(g.y)[(size_t)(row0 + r) * g.ldy + f] = from_f32<TY>(v);

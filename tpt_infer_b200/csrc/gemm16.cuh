@@ -78,13 +78,28 @@ __device__ __forceinline__ __half from_f32<__half>(float v) {
     return __float2half_rn(v);
 }
 
-// silu(x) = x / (1 + e^-x): for very negative x the quotient's denominator is
-// +inf and the result -0, the limit
-__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
-
-__device__ __forceinline__ float act16(float v, int act) {
-    if (act == TPT_ACT_SILU) return silu(v);
-    return apply_act(v, act);
+// The activations of the 16-bit products' epilogues, C values in place; act is
+// uniform, so the choice is one branch for all of them. Both smooth ones are
+// x / (1 + e^-z) with the hardware's exponential and quotient (errors of a few
+// 2^-22, far under the 16-bit rounding that follows): z = x for silu, and
+// z = 2 sqrt(2 / pi) (x + 0.044715 x^3) for gelu, since
+// 0.5 (1 + tanh(z / 2)) = 1 / (1 + e^-z). Far left e^-z is +inf and the
+// quotient -0, the limit. relu leaves NaN a NaN.
+template <int C>
+__device__ __forceinline__ void act16(float (&v)[C], int act) {
+    if (act == TPT_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < C; i++) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+    } else if (act == TPT_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < C; i++) {
+            const float z = v[i] * fmaf(0.0713548162726f * v[i], v[i], 1.5957691216057f);
+            v[i] = __fdividef(v[i], 1.0f + __expf(-z));
+        }
+    } else if (act == TPT_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < C; i++) v[i] = __fdividef(v[i], 1.0f + __expf(-v[i]));
+    }
 }
 
 #endif

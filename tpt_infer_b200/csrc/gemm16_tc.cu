@@ -129,50 +129,77 @@ __device__ __forceinline__ void commit_both(uint32_t bar) {
         : "memory");
 }
 
-// C columns (tokens col0 .. col0 + C - 1 of the tile) of this thread's lane.
-// Ungated: lane l of the warp is feature f0 + l. Gated: lanes l and l + 16 are
-// the gate and the up product of feature f0 + l; each of them finishes half of
-// the columns.
-template <typename T, typename TY, bool GATED, int C>
-__device__ __forceinline__ void epilogue16(const Args &a, float (&v)[C], int f0, size_t row0, int col0, int rows,
-                                           int lane) {
+// The epilogue of C columns (tokens col0 .. col0 + C - 1 of the tile) of this
+// thread's lane. Ungated: lane l of the warp is feature f0 + l, b its bias.
+// Gated: lanes l and l + 16 are the gate and the up product of feature f0 + l;
+// each of them finishes half of the columns. `acc` fills the accumulators; the
+// residual's loads are issued before it. A chunk whose columns are all rows
+// takes the branch-free path, so that its loads and stores go out back to back.
+template <typename TY, bool GATED, int C, typename Acc>
+__device__ __forceinline__ void epilogue16(const Args &a, float b, int f0, size_t row0, int col0, int rows, int lane,
+                                           Acc acc) {
+    float v[C];
     if constexpr (GATED) {
+        acc(v);
         const bool hi = lane >= 16;
         const int f = f0 + (lane & 15);
-        float h[C / 2];
+        float g[C / 2], u[C / 2];
 #pragma unroll
         for (int i = 0; i < C / 2; i++) {
             const float got = __shfl_xor_sync(0xffffffffu, hi ? v[i] : v[C / 2 + i], 16);
-            const float g = hi ? got : v[i], u = hi ? v[C / 2 + i] : got;
-            h[i] = act16(g, a.act) * u;
+            g[i] = hi ? got : v[i];
+            u[i] = hi ? v[C / 2 + i] : got;
         }
+        act16(g, a.act);
         const int c0 = col0 + (hi ? C / 2 : 0);
         TY *y = static_cast<TY *>(a.y) + (row0 + c0) * a.ldy + f;
-        if (f < a.n) {
+        const int n = f < a.n ? rows - c0 : 0;
+        if (n >= C / 2) {
 #pragma unroll
-            for (int i = 0; i < C / 2; i++)
-                if (c0 + i < rows) y[(size_t)i * a.ldy] = from_f32<TY>(h[i]);
+            for (int i = 0; i < C / 2; i++, y += a.ldy) *y = from_f32<TY>(g[i] * u[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < C / 2; i++, y += a.ldy)
+                if (i < n) *y = from_f32<TY>(g[i] * u[i]);
         }
     } else {
         const int f = f0 + lane;
-        if (f >= a.n) return;
-        const float b = a.bias ? to_f32(static_cast<const T *>(a.bias)[f]) : 0.0f;
-        TY *y = static_cast<TY *>(a.y) + (row0 + col0) * a.ldy + f;
+        const int n = f < a.n ? rows - col0 : 0;
+        TY rv[C];
         if (a.residual) {
             const TY *r = static_cast<const TY *>(a.residual) + (row0 + col0) * a.ldr + f;
-            float rv[C];
+            if (n >= C) {
 #pragma unroll
-            for (int i = 0; i < C; i++) rv[i] = col0 + i < rows ? to_f32(r[(size_t)i * a.ldr]) : 0.0f;
+                for (int i = 0; i < C; i++, r += a.ldr) rv[i] = *r;
+            } else {
 #pragma unroll
-            for (int i = 0; i < C; i++) v[i] = act16(v[i] + b, a.act) + rv[i];
+                for (int i = 0; i < C; i++, r += a.ldr) rv[i] = i < n ? *r : from_f32<TY>(0.0f);
+            }
+        }
+        acc(v);
+#pragma unroll
+        for (int i = 0; i < C; i++) v[i] += b;
+        act16(v, a.act);
+        if (a.residual) {
+#pragma unroll
+            for (int i = 0; i < C; i++) v[i] += to_f32(rv[i]);
+        }
+        TY *y = static_cast<TY *>(a.y) + (row0 + col0) * a.ldy + f;
+        if (n >= C) {
+#pragma unroll
+            for (int i = 0; i < C; i++, y += a.ldy) *y = from_f32<TY>(v[i]);
         } else {
 #pragma unroll
-            for (int i = 0; i < C; i++) v[i] = act16(v[i] + b, a.act);
+            for (int i = 0; i < C; i++, y += a.ldy)
+                if (i < n) *y = from_f32<TY>(v[i]);
         }
-#pragma unroll
-        for (int i = 0; i < C; i++)
-            if (col0 + i < rows) y[(size_t)i * a.ldy] = from_f32<TY>(v[i]);
     }
+    __syncwarp();
+}
+// the bias of feature f (0: none)
+template <typename T>
+__device__ __forceinline__ float bias_at(const Args &a, int f) {
+    return a.bias && f < a.n ? to_f32(static_cast<const T *>(a.bias)[f]) : 0.0f;
 }
 
 // ---------------------------------------------------------------------------
@@ -381,20 +408,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         uint32_t acc_phase = 0;
         for (int t = cluster; t < ntiles; t += nclusters) {
             const TileAt tl = tile_at(a, t);
+            const int f0 = GATED ? tl.ft * 128 + (int)rank * 64 + q * 16 : tl.ft * 256 + (int)rank * 128 + q * 32;
+            const float b = GATED ? 0.0f : bias_at<T>(a, f0 + lane);
             int okw = 0;
             if (lane == 0) okw = mbar_wait(tfull_bar(acc), acc_phase, abort_p, a.gflags, true) ? 1 : 0;
             okw = __shfl_sync(0xffffffffu, okw, 0);
             if (!okw) break;
             tc_fence_after();
-            const int f0 = GATED ? tl.ft * 128 + (int)rank * 64 + q * 16 : tl.ft * 256 + (int)rank * 128 + q * 32;
             const uint32_t t_base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 256);
 #pragma unroll 1
             for (int c = half * 32; c < tl.rows; c += 64) {
-                float v[32];
-                tmem_ld32(t_base + (uint32_t)c, reinterpret_cast<uint32_t(&)[32]>(v));
-                tmem_wait_ld();
-                epilogue16<T, TY, GATED, 32>(a, v, f0, (size_t)tl.row0, c, tl.rows, lane);
-                __syncwarp();
+                epilogue16<TY, GATED, 32>(a, b, f0, (size_t)tl.row0, c, tl.rows, lane, [&](float(&v)[32]) {
+                    tmem_ld32(t_base + (uint32_t)c, reinterpret_cast<uint32_t(&)[32]>(v));
+                    tmem_wait_ld();
+                });
             }
             tc_fence_before();
             __syncwarp();
@@ -567,6 +594,9 @@ __global__ void __launch_bounds__(S_THREADS, 2)
             }
         }
         // ---------------- epilogue (warps 2 to 5) ----------------
+        const int q = warp & 3;
+        const int f0 = GATED ? ft * 64 + q * 16 : ft * 128 + q * 32;
+        const float b = GATED ? 0.0f : bias_at<T>(a, f0 + lane);
         int go = 0;
         if (warp >= 2) {
             if (lane == 0) go = mbar_wait(done_bar, 0, abort_p, a.gflags, true) ? 1 : 0;
@@ -574,22 +604,19 @@ __global__ void __launch_bounds__(S_THREADS, 2)
             tc_fence_after();
         }
         __syncwarp();
-        const int q = warp & 3;
-        const int f0 = GATED ? ft * 64 + q * 16 : ft * 128 + q * 32;
         const uint32_t t_base = tmem + ((uint32_t)(q * 32) << 16);
         if constexpr (KS == 1) {
             if (go) {
                 constexpr int C = NT < 32 ? NT : 32;
 #pragma unroll 1
                 for (int c = 0; c < NT && c < rows; c += C) {
-                    float v[C];
-                    if constexpr (C == 32)
-                        tmem_ld32(t_base + (uint32_t)c, reinterpret_cast<uint32_t(&)[32]>(v));
-                    else
-                        tmem_ld16(t_base + (uint32_t)c, reinterpret_cast<uint32_t *>(v));
-                    tmem_wait_ld();
-                    epilogue16<T, TY, GATED, C>(a, v, f0, (size_t)row0, c, rows, lane);
-                    __syncwarp();
+                    epilogue16<TY, GATED, C>(a, b, f0, (size_t)row0, c, rows, lane, [&](float(&v)[C]) {
+                        if constexpr (C == 32)
+                            tmem_ld32(t_base + (uint32_t)c, reinterpret_cast<uint32_t(&)[32]>(v));
+                        else
+                            tmem_ld16(t_base + (uint32_t)c, reinterpret_cast<uint32_t *>(v));
+                        tmem_wait_ld();
+                    });
                 }
             }
         } else {
@@ -618,15 +645,14 @@ __global__ void __launch_bounds__(S_THREADS, 2)
                 constexpr int C = CW < 16 ? CW : 16;
 #pragma unroll 1
                 for (int c = 0; c < CW; c += C) {
-                    float v[C];
+                    epilogue16<TY, GATED, C>(a, b, f0, (size_t)row0, c0 + c, rows, lane, [&](float(&v)[C]) {
 #pragma unroll
-                    for (int i = 0; i < C; i++) {
-                        v[i] = part[(c + i) * W_ROWS];
+                        for (int i = 0; i < C; i++) {
+                            v[i] = part[(c + i) * W_ROWS];
 #pragma unroll
-                        for (int s = 1; s < KS; s++) v[i] += part[(s * CW + c + i) * W_ROWS];
-                    }
-                    epilogue16<T, TY, GATED, C>(a, v, f0, (size_t)row0, c0 + c, rows, lane);
-                    __syncwarp();
+                            for (int s = 1; s < KS; s++) v[i] += part[(s * CW + c + i) * W_ROWS];
+                        }
+                    });
                 }
             }
         }
