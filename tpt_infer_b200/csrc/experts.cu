@@ -187,20 +187,31 @@ void launch_route(tpt_cuda_ctx *ctx, const void *logits, size_t ld, int tokens, 
 // ------------------------------------------------------------------ the slots
 
 // Sorts the (token, choice) pairs by expert: pos[i] is pair i's slot (-1: no
-// expert), row_token[slot] its token; tiles lists each expert's slots in runs
-// of at most tile_rows. One block.
-__global__ void __launch_bounds__(1024)
-    k_experts_plan(const int *__restrict__ ids, int pairs, int top_k, int experts, int tile_rows, int *__restrict__ pos,
-                   int *__restrict__ row_token, Tile16 *__restrict__ tiles, int *__restrict__ n_tiles,
-                   unsigned *gflags) {
+// expert), row_token[slot] its token (null: not wanted); tiles lists each
+// expert's slots in runs of at most tile_rows, an expert's runs of equal
+// length up to the step that the product kernels count columns in.
+// One cluster of CL blocks: each counts its share of the pairs in shared
+// memory, the blocks add one another's counts, and each places its share.
+constexpr int PLAN_T = 1024;
+
+template <int CL>
+__global__ void __launch_bounds__(PLAN_T)
+    k_experts_plan(const int *__restrict__ ids, int pairs, int top_k, int experts, int tile_rows, int step, int *pos,
+                   int *row_token, Tile16 *tiles, int *n_tiles, unsigned *gflags) {
     extern __shared__ int plan_smem[];
     int *count = plan_smem, *first = plan_smem + experts;
+    __shared__ int warp_slots[PLAN_T / 32], warp_tiles[PLAN_T / 32];
+    __shared__ int run_slots, run_tiles;
+    const int rank = CL > 1 ? (int)tc::cluster_rank() : 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int e = threadIdx.x; e < experts; e += PLAN_T) count[e] = 0;
+    if (threadIdx.x == 0) run_slots = run_tiles = 0;
     pdl_wait();
     pdl_trigger();
-    for (int e = threadIdx.x; e < experts; e += 1024) count[e] = 0;
     __syncthreads();
+    const int i0 = (int)((long long)pairs * rank / CL), i1 = (int)((long long)pairs * (rank + 1) / CL);
     bool bad = false;
-    for (int i = threadIdx.x; i < pairs; i += 1024) {
+    for (int i = i0 + threadIdx.x; i < i1; i += PLAN_T) {
         const int e = ids[i];
         if (e >= experts)
             bad = true;
@@ -208,91 +219,273 @@ __global__ void __launch_bounds__(1024)
             atomicAdd(&count[e], 1);
     }
     if (bad) atomicOr(gflags + TPT_FLAG_CHECK, 1u);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int at = 0, nt = 0;
-        for (int e = 0; e < experts; e++) {
-            first[e] = at;
-            for (int r = 0; r < count[e]; r += tile_rows)
-                tiles[nt++] = Tile16{e, at + r, min(tile_rows, count[e] - r), 0};
-            at += count[e];
+    if (CL > 1)
+        tc::cluster_sync();
+    else
+        __syncthreads();
+    // first[e]: the first slot of this block's pairs of expert e. Exclusive sums
+    // over the experts, PLAN_T at a time; block 0 writes the tiles on the way.
+    for (int e0 = 0; e0 < experts; e0 += PLAN_T) {
+        const int e = e0 + threadIdx.x;
+        int total = 0, before = 0;
+        if (e < experts) {
+            if (CL > 1) {
+                const uint32_t at = tc::smem_u32(count + e);
+#pragma unroll
+                for (int r = 0; r < CL; r++) {
+                    int v;
+                    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(tc::map_to_rank(at, (uint32_t)r)) : "memory");
+                    if (r < rank) before += v;
+                    total += v;
+                }
+            } else {
+                total = count[e];
+            }
         }
-        *n_tiles = nt;
+        const int nt = (total + tile_rows - 1) / tile_rows;
+        int s = total, n = nt;  // inclusive sums over the warp
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int ps = __shfl_up_sync(0xffffffffu, s, o), pn = __shfl_up_sync(0xffffffffu, n, o);
+            if (lane >= o) {
+                s += ps;
+                n += pn;
+            }
+        }
+        if (lane == 31) {
+            warp_slots[warp] = s;
+            warp_tiles[warp] = n;
+        }
+        __syncthreads();
+        int ws = run_slots, wn = run_tiles;
+        for (int w = 0; w < warp; w++) {
+            ws += warp_slots[w];
+            wn += warp_tiles[w];
+        }
+        const int at = ws + s - total;
+        if (e < experts) first[e] = at + before;
+        if (rank == 0 && nt > 0) {
+            int each = (total + nt - 1) / nt;
+            each = (each + step - 1) / step * step;
+            for (int r = 0, k = wn + n - nt; r < nt; r++, k++) {
+                const int r0 = r * each;  // rounding up to the step can leave the last runs empty
+                tiles[k] = Tile16{e, at + min(r0, total), max(0, min(each, total - r0)), 0};
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x == PLAN_T - 1) {
+            run_slots = ws + s;
+            run_tiles = wn + n;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < pairs; i += 1024) {
+    if (rank == 0 && threadIdx.x == 0) *n_tiles = run_tiles;
+    for (int i = i0 + threadIdx.x; i < i1; i += PLAN_T) {
         const int e = ids[i];
         int slot = -1;
         if (e >= 0 && e < experts) {
             slot = atomicAdd(&first[e], 1);
-            row_token[slot] = i / top_k;
+            if (row_token) row_token[slot] = i / top_k;
         }
         pos[i] = slot;
     }
+    if (CL > 1) tc::cluster_sync();  // the counts are read by the other blocks
 }
 
-// y[t, d] = r[t, d] + sum_j w[t, j] P[pos[t, j], d], j in order
-template <typename T>
+// xs[pos[t, j], :] = x[t, :] for every choice j: each token's row is read once
+// and written to its slots, the rows padded to lds (a multiple of 8) with zeros.
+template <typename V>
 __global__ void __launch_bounds__(256)
-    k_experts_combine(const float *__restrict__ p, const int *__restrict__ pos, const float *__restrict__ weights,
-                      int tokens, int top_k, int d, const T *residual, size_t ldr, T *y, size_t ldy) {
+    k_experts_spread(const V *__restrict__ x, size_t ldx, int tokens, int d, const int *pos, int top_k, V *xs,
+                     size_t lds) {
     pdl_wait();
     pdl_trigger();
-    for (int t = blockIdx.x; t < tokens; t += gridDim.x)
-        for (int i = threadIdx.x; i < d; i += 256) {
-            float v = 0.0f;
+    for (int t = blockIdx.y; t < tokens; t += gridDim.y) {
+        const int *p = pos + (size_t)t * top_k;
+        for (int i = blockIdx.x * 256 + threadIdx.x; i < (int)lds; i += gridDim.x * 256) {
+            V v = {};
+            if (i < d) v = x[(size_t)t * ldx + i];
             for (int j = 0; j < top_k; j++) {
-                const int s = pos[(size_t)t * top_k + j];
-                if (s >= 0) v = fmaf(weights[(size_t)t * top_k + j], p[(size_t)s * d + i], v);
+                const int s = __ldcg(p + j);
+                if (s >= 0) xs[(size_t)s * lds + i] = v;
             }
-            if (residual) v += to_f32(residual[(size_t)t * ldr + i]);
-            y[(size_t)t * ldy + i] = from_f32<T>(v);
         }
+    }
 }
 
-// The products' intermediate results of one chunk of tokens stay under this
-// many bytes of workspace.
+// y[t, i] = r[t, i] + sum_j w[t, j] P[pos[t, j], i], j in order; V consecutive
+// values per thread, the rows of up to eight choices in flight together.
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+    k_experts_combine(const float *p, size_t ldp, const int *pos, const float *__restrict__ weights, int tokens,
+                      int top_k, int d, const T *residual, size_t ldr, T *y, size_t ldy) {
+    pdl_wait();
+    pdl_trigger();
+    for (int t = blockIdx.y; t < tokens; t += gridDim.y) {
+        const int *ps = pos + (size_t)t * top_k;
+        const float *w = weights + (size_t)t * top_k;
+        for (int i = (blockIdx.x * 256 + threadIdx.x) * V; i < d; i += gridDim.x * 256 * V) {
+            float v[V] = {};
+            for (int j0 = 0; j0 < top_k; j0 += 8) {
+                int s[8];
+                float wj[8], pv[8][V];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    s[j] = j0 + j < top_k ? __ldcg(ps + j0 + j) : -1;
+                    wj[j] = j0 + j < top_k ? w[j0 + j] : 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (s[j] < 0) continue;
+                    const float *row = p + (size_t)s[j] * ldp + i;
+                    if constexpr (V == 4) {
+                        const float4 q = __ldcs(reinterpret_cast<const float4 *>(row));
+                        pv[j][0] = q.x;
+                        pv[j][1] = q.y;
+                        pv[j][2] = q.z;
+                        pv[j][3] = q.w;
+                    } else {
+                        pv[j][0] = __ldcs(row);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (s[j] < 0) continue;
+#pragma unroll
+                    for (int c = 0; c < V; c++) v[c] = fmaf(wj[j], pv[j][c], v[c]);
+                }
+            }
+            const T *r = residual ? residual + (size_t)t * ldr + i : nullptr;
+            T *o = y + (size_t)t * ldy + i;
+            if constexpr (V == 4) {
+                union {
+                    uint2 u;
+                    T t[4];
+                } a, b;
+                if (r) {
+                    b.u = *reinterpret_cast<const uint2 *>(r);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) v[c] += to_f32(b.t[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; c++) a.t[c] = from_f32<T>(v[c]);
+                *reinterpret_cast<uint2 *>(o) = a.u;
+            } else {
+                if (r) v[0] += to_f32(*r);
+                *o = from_f32<T>(v[0]);
+            }
+        }
+    }
+}
+
+// The intermediate results of one chunk of tokens stay under this many bytes
+// of workspace.
 constexpr size_t EXPERTS_WS_BYTES = (size_t)2 << 30;
 
 template <typename T>
 int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tokens, size_t d, const int *ids,
                 const float *weights, size_t top_k, const T *w_in, const T *w_out, size_t experts, size_t f, int act,
                 bool gated, const T *residual, size_t ldr, T *y, size_t ldy) {
-    const size_t ldh = (f + 7) / 8 * 8;  // rows of h start on 16 bytes
-    const size_t per_token = top_k * (ldh * 2 + d * 4 + 8);
+    auto up8 = [](size_t v) { return (v + 7) / 8 * 8; };
+    const size_t ldh = up8(f), lds = up8(d), ldp = (d + 3) / 4 * 4;  // rows start on 16 bytes
+    // Tokens per tile of the products: what an expert gets on average, up to the
+    // pair kernel's 256 columns.
+    const size_t mean = (tokens * top_k + experts - 1) / experts;
+    const int tile_rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
+    const bool x_ok = ((uintptr_t)x & 15) == 0 && d % 8 == 0 && (tokens == 1 || ldx % 8 == 0);
+    // Up to 16 tokens per tile the product gathers x's rows itself (TMA, four
+    // rows an instruction, ~20 cycles a row): no launch and no copy. Longer
+    // tiles would wait for those rows, and x is spread over the slots first.
+    const bool gather = x_ok && tile_rows == 16;
+    const T *w_src[2] = {w_in, w_out};
+    const size_t w_rows[2] = {experts * (gated ? 2 : 1) * f, experts * d}, w_k[2] = {d, f};
+    bool pad[2];
+    size_t off = 0, o_w[2] = {0, 0};
+    auto take = [&](size_t bytes) {
+        const size_t at = off;
+        off += Staging::align_up(bytes);
+        return at;
+    };
+    for (int i = 0; i < 2; i++) {
+        pad[i] = !rows16_ok(w_src[i], w_k[i], w_rows[i]);
+        if (pad[i]) o_w[i] = take(w_rows[i] * up8(w_k[i]) * 2);
+    }
+    const size_t per_token = top_k * (ldh * 2 + ldp * 4 + (gather ? 0 : lds * 2) + 8);
     size_t chunk = EXPERTS_WS_BYTES / per_token;
     if (chunk < 1) chunk = 1;
     if (chunk > tokens) chunk = tokens;
-    // tokens per tile: what an expert gets on average, up to the pair kernel's 256
-    const size_t mean = (tokens * top_k + experts - 1) / experts;
-    const int tile_rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
+    const size_t max_pairs = chunk * top_k;
+    const size_t max_tiles = max_pairs / tile_rows + (max_pairs < experts ? max_pairs : experts);
+    const size_t o_pos = take(max_pairs * 4), o_tok = take(gather ? max_pairs * 4 : 0),
+                 o_tiles = take(max_tiles * sizeof(Tile16)), o_n = take(4),
+                 o_x = take(gather ? 0 : max_pairs * lds * 2), o_h = take(max_pairs * ldh * 2),
+                 o_p = take(max_pairs * ldp * 4);
+    int st = ensure_ws(ctx, off);
+    if (st) return st;
+    const void *w_use[2];
+    size_t w_ld[2];
+    for (int i = 0; i < 2; i++) {
+        w_use[i] = pad[i] ? (const void *)(ctx->ws + o_w[i]) : (const void *)w_src[i];
+        w_ld[i] = pad[i] ? up8(w_k[i]) : w_k[i];
+        if (pad[i]) {
+            st = launch_pad_rows16(ctx, w_src[i], w_k[i], w_rows[i], w_k[i], ctx->ws + o_w[i]);
+            if (st) return st;
+        }
+    }
+    int *pos = (int *)(ctx->ws + o_pos), *tok = gather ? (int *)(ctx->ws + o_tok) : nullptr;
+    int *n_tiles = (int *)(ctx->ws + o_n);
+    Tile16 *tiles = (Tile16 *)(ctx->ws + o_tiles);
+    float *p = (float *)(ctx->ws + o_p);
     for (size_t t0 = 0; t0 < tokens; t0 += chunk) {
         const size_t tn = tokens - t0 < chunk ? tokens - t0 : chunk;
         const size_t pairs = tn * top_k;
-        const size_t max_tiles = pairs / tile_rows + (pairs < experts ? pairs : experts);
-        size_t off = 0;
-        auto take = [&](size_t bytes) {
-            const size_t at = off;
-            off += Staging::align_up(bytes);
-            return at;
+        const T *xt = x + t0 * ldx;
+        // one block places up to 8192 pairs in about the time that a cluster of
+        // eight takes to meet
+        auto plan = [&](auto kern, int cl) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(cl);
+            cfg.blockDim = dim3(PLAN_T);
+            cfg.dynamicSmemBytes = experts * 8;
+            cfg.stream = ctx->stream;
+            cudaLaunchAttribute at[2];
+            at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            at[0].val.programmaticStreamSerializationAllowed = 1;
+            at[1].id = cudaLaunchAttributeClusterDimension;
+            at[1].val.clusterDim.x = cl;
+            at[1].val.clusterDim.y = 1;
+            at[1].val.clusterDim.z = 1;
+            cfg.attrs = at;
+            cfg.numAttrs = cl > 1 ? 2 : 1;
+            (void)cudaLaunchKernelEx(&cfg, kern, ids + t0 * top_k, (int)pairs, (int)top_k, (int)experts, tile_rows,
+                                     tile_rows == 256 ? 32 : 16, pos, tok, tiles, n_tiles, ctx->d_flags);
         };
-        const size_t o_pos = take(pairs * 4), o_tok = take(pairs * 4), o_tiles = take(max_tiles * sizeof(Tile16)),
-                     o_n = take(4), o_h = take(pairs * ldh * 2), o_p = take(pairs * d * 4);
-        int st = ensure_ws(ctx, off);
-        if (st) return st;
-        int *pos = (int *)(ctx->ws + o_pos), *tok = (int *)(ctx->ws + o_tok), *n_tiles = (int *)(ctx->ws + o_n);
-        Tile16 *tiles = (Tile16 *)(ctx->ws + o_tiles);
-        launch_pdl(k_experts_plan, 1, 1024, experts * 8, ctx->stream, ids + t0 * top_k, (int)pairs, (int)top_k,
-                   (int)experts, tile_rows, pos, tok, tiles, n_tiles, ctx->d_flags);
+        if (pairs <= 8192)
+            plan(k_experts_plan<1>, 1);
+        else
+            plan(k_experts_plan<8>, 8);
         st = after_launch(ctx, "experts_plan");
         if (st) return st;
+        if (!gather) {
+            const unsigned rows = (unsigned)(tn < 16384 ? tn : 16384);
+            if (x_ok)
+                launch_pdl(k_experts_spread<uint4>, dim3((unsigned)((lds / 8 + 255) / 256), rows), 256, 0, ctx->stream,
+                           (const uint4 *)xt, ldx / 8, (int)tn, (int)(d / 8), pos, (int)top_k, (uint4 *)(ctx->ws + o_x),
+                           lds / 8);
+            else
+                launch_pdl(k_experts_spread<uint16_t>, dim3((unsigned)((lds + 255) / 256), rows), 256, 0, ctx->stream,
+                           (const uint16_t *)xt, ldx, (int)tn, (int)d, pos, (int)top_k, (uint16_t *)(ctx->ws + o_x),
+                           lds);
+            st = after_launch(ctx, "experts_spread");
+            if (st) return st;
+        }
         Gemm16 g;
-        g.x = x + t0 * ldx;
-        g.ldx = ldx;
-        g.x_rows = (int)tn;
-        g.w = w_in;
-        g.ldw = d;
-        g.w_expert = (gated ? 2 : 1) * f * d;
+        g.x = gather ? (const void *)xt : (const void *)(ctx->ws + o_x);
+        g.ldx = gather ? ldx : lds;
+        g.x_rows = (int)(gather ? tn : pairs);
+        g.w = w_use[0];
+        g.ldw = w_ld[0];
+        g.w_expert = (gated ? 2 : 1) * f * w_ld[0];
         g.rows = (int)pairs;
         g.n = (int)f;
         g.k = (int)d;
@@ -300,7 +493,7 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
         g.row_token = tok;
         g.tiles = tiles;
         g.n_tiles = n_tiles;
-        g.max_tiles = (int)max_tiles;
+        g.max_tiles = (int)(pairs / tile_rows + (pairs < experts ? pairs : experts));
         g.tile_rows = tile_rows;
         g.act = act;
         g.gated = gated;
@@ -312,25 +505,33 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
         o.x = g.y;
         o.ldx = ldh;
         o.x_rows = (int)pairs;
-        o.w = w_out;
-        o.ldw = f;
-        o.w_expert = d * f;
+        o.w = w_use[1];
+        o.ldw = w_ld[1];
+        o.w_expert = d * w_ld[1];
         o.rows = (int)pairs;
         o.n = (int)d;
         o.k = (int)f;
         o.experts = (int)experts;
         o.tiles = tiles;
         o.n_tiles = n_tiles;
-        o.max_tiles = (int)max_tiles;
+        o.max_tiles = g.max_tiles;
         o.tile_rows = tile_rows;
-        o.y = ctx->ws + o_p;
-        o.ldy = d;
+        o.y = p;
+        o.ldy = ldp;
         o.y_f32 = true;
         st = launch_gemm16(ctx, dtype, o);
         if (st) return st;
-        launch_pdl(k_experts_combine<T>, (unsigned)(tn < 148 * 16 ? tn : 148 * 16), 256, 0, ctx->stream,
-                   (const float *)(ctx->ws + o_p), pos, weights + t0 * top_k, (int)tn, (int)top_k, (int)d,
-                   residual ? residual + t0 * ldr : nullptr, ldr, y + t0 * ldy, ldy);
+        const T *rt = residual ? residual + t0 * ldr : nullptr;
+        T *yt = y + t0 * ldy;
+        const bool vec = d % 4 == 0 && ldy % 4 == 0 && ((uintptr_t)yt & 7) == 0 &&
+                         (!rt || (ldr % 4 == 0 && ((uintptr_t)rt & 7) == 0));
+        const unsigned rows = (unsigned)(tn < 16384 ? tn : 16384);
+        if (vec)
+            launch_pdl(k_experts_combine<T, 4>, dim3((unsigned)((d + 1023) / 1024), rows), 256, 0, ctx->stream, p, ldp,
+                       pos, weights + t0 * top_k, (int)tn, (int)top_k, (int)d, rt, ldr, yt, ldy);
+        else
+            launch_pdl(k_experts_combine<T, 1>, dim3((unsigned)((d + 255) / 256), rows), 256, 0, ctx->stream, p, ldp,
+                       pos, weights + t0 * top_k, (int)tn, (int)top_k, (int)d, rt, ldr, yt, ldy);
         st = after_launch(ctx, "experts_combine");
         if (st) return st;
     }

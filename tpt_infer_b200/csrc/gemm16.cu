@@ -1,108 +1,28 @@
-// gemm16.cu -- 16-bit matrix products with their epilogue: the linear layer
-// y = act(x w^T + bias) + residual, and one of the experts' products over a
-// schedule of (expert, rows) tiles.
+// gemm16.cu -- the 16-bit linear layer y = act(x w^T + bias) + residual: its
+// entry point, and the copies of operands whose rows TMA cannot read.
 #include "gemm16.cuh"
 
 namespace tpt {
 namespace {
 
-constexpr int SB = 64, SK = 16;  // output tile, k step
-
-// 64 x 64 outputs per block of 256 threads, 4 x 4 per thread, f32 sums.
-// gridDim.x: feature tiles; gridDim.y: row tiles (dense) or schedule tiles.
-template <typename T, typename TY, bool GATED>
-__global__ void __launch_bounds__(256) k_gemm16_simple(Gemm16 g) {
+__global__ void __launch_bounds__(256)
+    k_pad_rows16(const uint16_t *__restrict__ src, size_t ld, size_t rows, size_t k, uint16_t *dst, size_t k8) {
     pdl_wait();
     pdl_trigger();
-    __shared__ float xs[SK][SB + 4], ws[SK][SB + 4], us[GATED ? SK : 1][SB + 4];
-    int row0, rows, expert = 0;
-    if (g.tiles) {
-        const int sub = (g.tile_rows + SB - 1) / SB;
-        const int ti = blockIdx.y / sub, off = (blockIdx.y - ti * sub) * SB;
-        if (ti >= *g.n_tiles) return;
-        const Tile16 t = g.tiles[ti];
-        if (off >= t.rows) return;
-        row0 = t.row0 + off;
-        rows = min(SB, t.rows - off);
-        expert = t.expert;
-    } else {
-        row0 = blockIdx.y * SB;
-        rows = min(SB, g.rows - row0);
+    const size_t n = rows * k8;
+    for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const size_t r = i / k8, c = i - r * k8;
+        dst[i] = c < k ? src[r * ld + c] : (uint16_t)0;
     }
-    const int f0 = blockIdx.x * SB;
-    const T *x = static_cast<const T *>(g.x);
-    const T *w = static_cast<const T *>(g.w) + (size_t)expert * g.w_expert;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {}, up[4][4] = {};
-    for (int k0 = 0; k0 < g.k; k0 += SK) {
-        for (int i = threadIdx.x; i < SB * SK; i += 256) {
-            const int r = i / SK, c = i % SK;
-            const bool kin = k0 + c < g.k;
-            float v = 0.0f, a = 0.0f, u = 0.0f;
-            if (kin && r < rows) {
-                const size_t xr = g.row_token ? (size_t)g.row_token[row0 + r] : (size_t)(row0 + r);
-                v = to_f32(x[xr * g.ldx + k0 + c]);
-            }
-            if (kin && f0 + r < g.n) {
-                a = to_f32(w[(size_t)(f0 + r) * g.ldw + k0 + c]);
-                if (GATED) u = to_f32(w[(size_t)(g.n + f0 + r) * g.ldw + k0 + c]);
-            }
-            xs[c][r] = v;
-            ws[c][r] = a;
-            if (GATED) us[c][r] = u;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < SK; c++) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    acc[i][j] = fmaf(xs[c][ty * 4 + i], ws[c][tx * 4 + j], acc[i][j]);
-                    if (GATED) up[i][j] = fmaf(xs[c][ty * 4 + i], us[c][tx * 4 + j], up[i][j]);
-                }
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int r = ty * 4 + i;
-        if (r >= rows) continue;
-        if (g.bias) {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (f0 + tx * 4 + j < g.n) acc[i][j] += to_f32(static_cast<const T *>(g.bias)[f0 + tx * 4 + j]);
-        }
-        act16(acc[i], g.act);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int f = f0 + tx * 4 + j;
-            if (f >= g.n) continue;
-            float v = acc[i][j];
-            if (GATED) v *= up[i][j];
-            if (g.residual) v += to_f32(static_cast<const TY *>(g.residual)[(size_t)(row0 + r) * g.ldr + f]);
-            static_cast<TY *>(g.y)[(size_t)(row0 + r) * g.ldy + f] = from_f32<TY>(v);
-        }
-    }
-}
-
-template <typename T>
-int launch_simple(tpt_cuda_ctx *ctx, const Gemm16 &g) {
-    const dim3 grid((g.n + SB - 1) / SB, g.tiles ? g.max_tiles * ((g.tile_rows + SB - 1) / SB) : (g.rows + SB - 1) / SB);
-    if (g.gated)
-        launch_pdl(k_gemm16_simple<T, T, true>, grid, 256, 0, ctx->stream, g);
-    else if (g.y_f32)
-        launch_pdl(k_gemm16_simple<T, float, false>, grid, 256, 0, ctx->stream, g);
-    else
-        launch_pdl(k_gemm16_simple<T, T, false>, grid, 256, 0, ctx->stream, g);
-    return after_launch(ctx, "gemm16_simple");
 }
 
 }  // namespace
 
-int launch_gemm16(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
-    if (gemm16_tc_ok(g)) return launch_gemm16_tc(ctx, dtype, g);
-    return dtype == TPT_DT_BF16 ? launch_simple<__nv_bfloat16>(ctx, g) : launch_simple<__half>(ctx, g);
+int launch_pad_rows16(tpt_cuda_ctx *ctx, const void *src, size_t ld, size_t rows, size_t k, void *dst) {
+    const size_t k8 = k ? (k + 7) / 8 * 8 : 8;
+    launch_pdl(k_pad_rows16, grid_1d(rows * k8, 256), 256, 0, ctx->stream, (const uint16_t *)src, ld, rows, k,
+               (uint16_t *)dst, k8);
+    return after_launch(ctx, "pad_rows16");
 }
 
 }  // namespace tpt
@@ -141,6 +61,28 @@ int tpt_cuda_linear_dev(tpt_cuda_ctx *ctx, int dtype, const void *x, size_t ldx,
     g.y = y;
     g.ldy = ldy;
     g.y_f32 = y_dtype == TPT_DT_F32;
+    // TMA reads rows that start on 16 bytes; others are copied to the workspace
+    // first (k = 0 becomes eight zero products).
+    const size_t k8 = k ? (k + 7) / 8 * 8 : 8;
+    const bool px = k == 0 || !rows16_ok(x, ldx, m), pw = k == 0 || !rows16_ok(w, ldw, n);
+    const size_t xb = px ? Staging::align_up(m * k8 * 2) : 0, wb = pw ? n * k8 * 2 : 0;
+    if (px || pw) {
+        int st = ensure_ws(ctx, xb + wb);
+        if (st) return st;
+        if (px) {
+            st = launch_pad_rows16(ctx, x, ldx, m, k, ctx->ws);
+            if (st) return st;
+            g.x = ctx->ws;
+            g.ldx = k8;
+        }
+        if (pw) {
+            st = launch_pad_rows16(ctx, w, ldw, n, k, ctx->ws + xb);
+            if (st) return st;
+            g.w = ctx->ws + xb;
+            g.ldw = k8;
+        }
+        if (k == 0) g.k = 8;
+    }
     return launch_gemm16(ctx, dtype, g);
 }
 

@@ -41,11 +41,17 @@ struct Gemm16 {
     bool y_f32 = false;
 };
 
-// device enqueue; dtype TPT_DT_BF16 or TPT_DT_F16
+// Device enqueue; dtype TPT_DT_BF16 or TPT_DT_F16, k > 0. The operands' rows
+// must pass rows16_ok (the copies below make them).
 int launch_gemm16(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g);
-// the tensor-core kernels: whether TMA can read the operands, and the launch
-bool gemm16_tc_ok(const Gemm16 &g);
-int launch_gemm16_tc(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g);
+
+// Whether TMA can read `rows` rows of 16-bit values ld apart: base and rows on
+// 16 bytes.
+inline bool rows16_ok(const void *p, size_t ld, size_t rows) {
+    return ((uintptr_t)p & 15) == 0 && (rows <= 1 || ld % 8 == 0);
+}
+// dst [rows][k rounded up to a multiple of 8] = src [rows][k], zero-filled
+int launch_pad_rows16(tpt_cuda_ctx *ctx, const void *src, size_t ld, size_t rows, size_t k, void *dst);
 
 #ifdef __CUDACC__
 

@@ -35,7 +35,6 @@ struct Args {
     int rows, n, k;
     int ftiles;                  // feature tiles
     int tile_n;                  // dense: tokens per tile
-    int box_rows;                // X's box (no gather)
     int group;                   // dense: token tiles that share a sweep over the features
     uint32_t fmt;                // 0 f16, 1 bf16
     const int *row_token;
@@ -93,15 +92,6 @@ __device__ __forceinline__ void tma_load_4d_p(uint32_t dst, const CUtensorMap *t
         "r"(u)
         : "memory");
 }
-__device__ __forceinline__ void tma_gather4_p(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x,
-                                              const int (&r)[4]) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 "
-        "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
-        : "memory");
-}
-
 template <int GROUP>
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -248,7 +238,7 @@ __device__ __forceinline__ TileAt tile_at(const Args &a, int t) {
 template <typename T, typename TY, bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     k_gemm16_pair(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                  const __grid_constant__ Args a) {
+                  const __grid_constant__ CUtensorMap tmX16, const __grid_constant__ Args a) {
     constexpr int S = P_STAGES;
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag;
@@ -298,7 +288,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     const int ntiles = a.tiles ? __ldcg(a.n_tiles) * a.ftiles : ((a.rows + a.tile_n - 1) / a.tile_n) * a.ftiles;
 
     if (warp == 0) {
-        // ---------------- producer: lane 0 the boxes, every lane four gathered rows ----------------
+        if (lane == 0) {
+        // ---------------- producer ----------------
         int stage = 0;
         uint32_t phase = 0;
         int issued = 0;
@@ -308,36 +299,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             const int half = tl.cols >> 1;
             const uint32_t bytes = 2u * (W_BYTES + half * ROW_BYTES);
             const int xrow = tl.row0 + (int)rank * half;
-            int r4[4];
-            if (a.row_token) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {  // past the tile's rows: its first row, into columns that nothing reads
-                    const int c = (int)rank * half + lane * 4 + i;
-                    r4[i] = __ldcg(a.row_token + tl.row0 + (c < tl.rows ? c : 0));
-                }
-            }
+            const bool whole = half == a.tile_n / 2;  // one box holds this CTA's rows
             for (int kb = 0; kb < kblocks; kb++) {
-                if (lane == 0) ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_p, a.gflags, true);
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-                if (!ok) break;
+                if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_p, a.gflags, true)) {
+                    ok = false;
+                    break;
+                }
                 const uint32_t w_dst = ring + stage * P_STAGE_BYTES, x_dst = w_dst + W_BYTES;
                 const uint32_t fb = map_to_rank(full_bar(stage), 0);
-                if (lane == 0) {
-                    if (leader) mbar_arrive_expect_tx(full_bar(stage), bytes);
-                    if (GATED) {
+                if (leader) mbar_arrive_expect_tx(full_bar(stage), bytes);
+                if (GATED) {
 #pragma unroll
-                        for (int q = 0; q < 4; q++)
-                            tma_load_4d_p(w_dst + q * 4096, &tmW, fb, kb * BK, tl.ft * 128 + (int)rank * 64 + q * 16,
-                                          0, tl.expert);
-                    } else {
-                        tma_load_3d_p(w_dst, &tmW, fb, kb * BK, tl.ft * 256 + (int)rank * 128, tl.expert);
-                    }
-                    if (!a.row_token)
-                        for (int r = 0; r < half; r += a.box_rows)
-                            tma_load_2d_p(x_dst + r * ROW_BYTES, &tmX, fb, kb * BK, xrow + r);
+                    for (int q = 0; q < 4; q++)
+                        tma_load_4d_p(w_dst + q * 4096, &tmW, fb, kb * BK, tl.ft * 128 + (int)rank * 64 + q * 16, 0,
+                                      tl.expert);
+                } else {
+                    tma_load_3d_p(w_dst, &tmW, fb, kb * BK, tl.ft * 256 + (int)rank * 128, tl.expert);
                 }
-                __syncwarp();
-                if (a.row_token && lane * 4 < half) tma_gather4_p(x_dst + lane * 4 * ROW_BYTES, &tmX, fb, kb * BK, r4);
+                if (whole)
+                    tma_load_2d_p(x_dst, &tmX, fb, kb * BK, xrow);
+                else
+                    for (int r = 0; r < half; r += 16)
+                        tma_load_2d_p(x_dst + r * ROW_BYTES, &tmX16, fb, kb * BK, xrow + r);
                 issued++;
                 if (++stage == S) {
                     stage = 0;
@@ -347,7 +330,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         }
         // an aborting pair leaves no copy in flight behind it: the leader waits
         // (bounded) for the stages it announced and did not see consumed
-        if (!ok && leader && lane == 0) {
+        if (!ok && leader) {
             const int n = issued < S ? issued : S;
             for (int i = 0; i < n; i++) {
                 if (--stage < 0) {
@@ -356,6 +339,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                 }
                 mbar_wait(full_bar(stage), phase, abort_p, a.gflags, false);
             }
+        }
         }
     } else if (warp == 1) {
         if (lane == 0 && leader) {
@@ -760,15 +744,14 @@ int launch_pair(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g, int tile_n) {
     Args a = make_args(ctx, dtype, g);
     a.ftiles = (g.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
     a.tile_n = tile_n;
-    a.box_rows = g.tiles ? 16 : tile_n / 2;
     a.group = 8;
-    CUtensorMap tw, tx;
-    if (!weight_map(&tw, dtype, g) || !token_map(&tx, dtype, g, (unsigned)a.box_rows))
+    CUtensorMap tw, tx, tx16;
+    if (!weight_map(&tw, dtype, g) || !token_map(&tx, dtype, g, (unsigned)tile_n / 2) || !token_map(&tx16, dtype, g, 16))
         return cuda_fail(ctx, cudaErrorInvalidValue, "gemm16_pair tensor map");
     const long long tiles = (g.tiles ? (long long)g.max_tiles : ((long long)g.rows + tile_n - 1) / tile_n) * a.ftiles;
     if (tiles > 0x7fffffffLL) return TPT_UNSUPPORTED;
     const int clusters = tiles < pairs ? (int)tiles : pairs;
-    launch_pdl(kern, 2 * clusters, P_THREADS, P_SMEM, ctx->stream, tw, tx, a);
+    launch_pdl(kern, 2 * clusters, P_THREADS, P_SMEM, ctx->stream, tw, tx, tx16, a);
     return after_launch(ctx, "gemm16_pair");
 }
 
@@ -844,14 +827,7 @@ int launch_typed(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
 
 }  // namespace
 
-bool gemm16_tc_ok(const Gemm16 &g) {
-    auto al = [](const void *p) { return ((uintptr_t)p & 15) == 0; };
-    return g.k > 0 && al(g.x) && al(g.w) && (g.x_rows <= 1 || g.ldx % 8 == 0) &&
-           ((g.n <= 1 && !g.gated) || g.ldw % 8 == 0) &&
-           (!g.gated || ((size_t)g.n * g.ldw) % 8 == 0) && (g.experts <= 1 || g.w_expert % 8 == 0);
-}
-
-int launch_gemm16_tc(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
+int launch_gemm16(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
     return dtype == TPT_DT_BF16 ? launch_typed<__nv_bfloat16>(ctx, dtype, g) : launch_typed<__half>(ctx, dtype, g);
 }
 
