@@ -268,8 +268,10 @@ __global__ void __launch_bounds__(PLAN_T)
             int each = (total + nt - 1) / nt;
             each = (each + step - 1) / step * step;
             for (int r = 0, k = wn + n - nt; r < nt; r++, k++) {
-                const int r0 = r * each;  // rounding up to the step can leave the last runs empty
-                tiles[k] = Tile16{e, at + min(r0, total), max(0, min(each, total - r0)), 0};
+                // no tile is empty: (nt - 1) * each <= (nt - 1) * tile_rows < total
+                const int place = r % TILE_RUN;
+                tiles[k] = Tile16{e, at + r * each, min(each, total - r * each),
+                                  place << 8 | min(TILE_RUN, nt - (r - place))};
             }
         }
         __syncthreads();

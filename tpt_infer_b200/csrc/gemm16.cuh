@@ -15,8 +15,11 @@ namespace tpt {
 // up = W[n + f, :] x. Grouped: the rows of tile t go through the weight of
 // tiles[t].expert; X's row of a slot is row_token[slot] (the slot itself
 // without a list), Y's row is the slot.
+// An expert's tiles lie in runs of up to TILE_RUN: `run` holds the tile's place
+// in its run (from bit 8) and the run's length (8 bits).
+constexpr int TILE_RUN = 8;
 struct Tile16 {
-    int expert, row0, rows, pad;
+    int expert, row0, rows, run;
 };
 struct Gemm16 {
     const void *x = nullptr;

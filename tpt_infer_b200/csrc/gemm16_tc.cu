@@ -37,6 +37,7 @@ struct Args {
     int tile_n;                  // dense: tokens per tile
     int group;                   // dense: token tiles that share a sweep over the features
     uint32_t fmt;                // 0 f16, 1 bf16
+    int gate16;                  // gated: n is a multiple of 16 (see weight_map)
     const int *row_token;
     const Tile16 *tiles;
     const int *n_tiles;
@@ -92,6 +93,23 @@ __device__ __forceinline__ void tma_load_4d_p(uint32_t dst, const CUtensorMap *t
         "r"(u)
         : "memory");
 }
+__device__ __forceinline__ void tma_load_5d_p(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, int y, int z,
+                                              int u, int v) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+        "{%3, %4, %5, %6, %7}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y),
+        "r"(z), "r"(u), "r"(v)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, int y, int z,
+                                            int u, int v) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, "
+        "%6, %7}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u),
+        "r"(v)
+        : "memory");
+}
+
 template <int GROUP>
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -205,17 +223,28 @@ constexpr int P_EPI_WARPS = 8;
 constexpr int P_THREADS = (2 + P_EPI_WARPS) * 32;
 constexpr int P_SMEM = P_STAGES * P_STAGE_BYTES + (2 * P_STAGES + 5) * 8 + 1024;
 
+// X's maps with boxes of 128, 64 and 32 rows: a stage's token rows are one box,
+// the smallest that holds them. (Rows past the tile land in columns that nothing
+// reads; a box costs the issuing thread more than its extra rows cost the L2.)
+struct XMaps {
+    CUtensorMap box[3];
+};
 struct TileAt {
     int expert, row0, rows, cols, ft;
 };
-// Tile t of the product. Dense: sweeps of `group` token tiles over all the
-// features, so that the tiles in flight share both operands in L2.
+// Tile t of the product: sweeps of several token tiles over all the features, so
+// that the tiles in flight share both operands in L2. Dense: `group` token tiles
+// a sweep; grouped: the schedule's runs of tiles of one expert (a run's tiles and
+// its feature tiles take the same place in the order of t as tile by tile).
 __device__ __forceinline__ TileAt tile_at(const Args &a, int t) {
     TileAt r;
     if (a.tiles) {
+        const int4 *tiles = reinterpret_cast<const int4 *>(a.tiles);
         const int i = t / a.ftiles;
-        r.ft = t - i * a.ftiles;
-        const int4 q = __ldcg(reinterpret_cast<const int4 *>(a.tiles) + i);
+        const int run = __ldcg(tiles + i).w, place = run >> 8, wide = run & 255;
+        const int in = t - (i - place) * a.ftiles;
+        r.ft = in / wide;
+        const int4 q = __ldcg(tiles + (i - place) + in - r.ft * wide);
         r.expert = q.x;
         r.row0 = q.y;
         r.rows = q.z;
@@ -237,8 +266,8 @@ __device__ __forceinline__ TileAt tile_at(const Args &a, int t) {
 
 template <typename T, typename TY, bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
-    k_gemm16_pair(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                  const __grid_constant__ CUtensorMap tmX16, const __grid_constant__ Args a) {
+    k_gemm16_pair(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ XMaps tmX,
+                  const __grid_constant__ Args a) {
     constexpr int S = P_STAGES;
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag;
@@ -270,7 +299,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         mbar_init(drain_bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmW)) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX.box[0])) : "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
@@ -297,9 +326,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         for (int t = cluster; t < ntiles && ok; t += nclusters) {
             const TileAt tl = tile_at(a, t);
             const int half = tl.cols >> 1;
-            const uint32_t bytes = 2u * (W_BYTES + half * ROW_BYTES);
+            const int box = half > 64 ? 0 : half > 32 ? 1 : 2;
+            const uint32_t bytes = 2u * (W_BYTES + (W_BYTES >> box));
             const int xrow = tl.row0 + (int)rank * half;
-            const bool whole = half == a.tile_n / 2;  // one box holds this CTA's rows
             for (int kb = 0; kb < kblocks; kb++) {
                 if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_p, a.gflags, true)) {
                     ok = false;
@@ -308,7 +337,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                 const uint32_t w_dst = ring + stage * P_STAGE_BYTES, x_dst = w_dst + W_BYTES;
                 const uint32_t fb = map_to_rank(full_bar(stage), 0);
                 if (leader) mbar_arrive_expect_tx(full_bar(stage), bytes);
-                if (GATED) {
+                if (GATED && a.gate16) {
+                    tma_load_5d_p(w_dst, &tmW, fb, kb * BK, 0, 0, tl.ft * 8 + (int)rank * 4, tl.expert);
+                } else if (GATED) {
 #pragma unroll
                     for (int q = 0; q < 4; q++)
                         tma_load_4d_p(w_dst + q * 4096, &tmW, fb, kb * BK, tl.ft * 128 + (int)rank * 64 + q * 16, 0,
@@ -316,11 +347,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                 } else {
                     tma_load_3d_p(w_dst, &tmW, fb, kb * BK, tl.ft * 256 + (int)rank * 128, tl.expert);
                 }
-                if (whole)
-                    tma_load_2d_p(x_dst, &tmX, fb, kb * BK, xrow);
-                else
-                    for (int r = 0; r < half; r += 16)
-                        tma_load_2d_p(x_dst + r * ROW_BYTES, &tmX16, fb, kb * BK, xrow + r);
+                tma_load_2d_p(x_dst, &tmX.box[box], fb, kb * BK, xrow);
                 issued++;
                 if (++stage == S) {
                     stage = 0;
@@ -526,7 +553,9 @@ __global__ void __launch_bounds__(S_THREADS, 2)
                 const uint32_t fb = full_bar(stage);
                 if (lane == 0) {
                     mbar_arrive_expect_tx(fb, Cfg::STAGE_BYTES);
-                    if (GATED) {
+                    if (GATED && a.gate16) {
+                        tma_load_5d(w_dst, &tmW, fb, kb * BK, 0, 0, ft * 4, expert);
+                    } else if (GATED) {
 #pragma unroll
                         for (int q = 0; q < 4; q++)
                             tma_load_4d(w_dst + q * 4096, &tmW, fb, kb * BK, ft * 64 + q * 16, 0, expert);
@@ -660,8 +689,8 @@ bool make_map(CUtensorMap *tm, int dtype, const void *base, int rank, const size
               const unsigned *box) {
     auto fn = encode_fn();
     if (!fn || ((uintptr_t)base & 15)) return false;
-    cuuint64_t d[4], s[3];
-    cuuint32_t b[4], e[4] = {1, 1, 1, 1};
+    cuuint64_t d[5], s[4];
+    cuuint32_t b[5], e[5] = {1, 1, 1, 1, 1};
     for (int i = 0; i < rank; i++) {
         d[i] = dims[i];
         b[i] = box[i];
@@ -679,6 +708,16 @@ bool make_map(CUtensorMap *tm, int dtype, const void *base, int rank, const size
 bool weight_map(CUtensorMap *tm, int dtype, const Gemm16 &g) {
     const size_t ldw = g.n > 1 || g.gated ? g.ldw : (size_t)(g.k + 7) / 8 * 8;
     const size_t we = g.experts > 1 ? g.w_expert : (size_t)(g.gated ? 2 : 1) * g.n * ldw;
+    // Gated: a tile's rows are 16 gate rows, the 16 up rows of the same features,
+    // and so on. With n a multiple of 16 the features are a dimension of 16 and
+    // one of n / 16, and one box brings all 128 rows; otherwise a box of 16 + 16
+    // rows whose feature dimension ends at n (rows past it read as zero).
+    if (g.gated && g.n % 16 == 0) {
+        const size_t dims[5] = {(size_t)g.k, 16, 2, (size_t)g.n / 16, (size_t)g.experts};
+        const size_t st[4] = {ldw, (size_t)g.n * ldw, 16 * ldw, we};
+        const unsigned box[5] = {BK, 16, 2, 4, 1};
+        return make_map(tm, dtype, g.w, 5, dims, st, box);
+    }
     if (g.gated) {
         const size_t dims[4] = {(size_t)g.k, (size_t)g.n, 2, (size_t)g.experts}, st[3] = {ldw, (size_t)g.n * ldw, we};
         const unsigned box[4] = {BK, 16, 2, 1};
@@ -701,6 +740,7 @@ Args make_args(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
     a.n = g.n;
     a.k = g.k;
     a.fmt = dtype == TPT_DT_BF16 ? 1 : 0;
+    a.gate16 = g.n % 16 == 0;
     a.row_token = g.row_token;
     a.tiles = g.tiles;
     a.n_tiles = g.n_tiles;
@@ -745,13 +785,15 @@ int launch_pair(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g, int tile_n) {
     a.ftiles = (g.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
     a.tile_n = tile_n;
     a.group = 8;
-    CUtensorMap tw, tx, tx16;
-    if (!weight_map(&tw, dtype, g) || !token_map(&tx, dtype, g, (unsigned)tile_n / 2) || !token_map(&tx16, dtype, g, 16))
+    CUtensorMap tw;
+    XMaps tx;
+    if (!weight_map(&tw, dtype, g) || !token_map(&tx.box[0], dtype, g, 128) || !token_map(&tx.box[1], dtype, g, 64) ||
+        !token_map(&tx.box[2], dtype, g, 32))
         return cuda_fail(ctx, cudaErrorInvalidValue, "gemm16_pair tensor map");
     const long long tiles = (g.tiles ? (long long)g.max_tiles : ((long long)g.rows + tile_n - 1) / tile_n) * a.ftiles;
     if (tiles > 0x7fffffffLL) return TPT_UNSUPPORTED;
     const int clusters = tiles < pairs ? (int)tiles : pairs;
-    launch_pdl(kern, 2 * clusters, P_THREADS, P_SMEM, ctx->stream, tw, tx, tx16, a);
+    launch_pdl(kern, 2 * clusters, P_THREADS, P_SMEM, ctx->stream, tw, tx, a);
     return after_launch(ctx, "gemm16_pair");
 }
 
