@@ -22,6 +22,7 @@ OK, SIZE_MISMATCH, SHAPE_MISMATCH, UNSUPPORTED, INVALID = 0, 1, 2, 3, 4
 CUDA_ERROR, OUT_OF_MEMORY, TIMEOUT, NCCL_ERROR, DEVICE_CHECK = 5, 6, 7, 8, 9
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
 DT_F32, DT_BF16, DT_F16 = 0, 2, 3
+_I32, _U8 = 100, 101
 _SCORES = {"softmax": 0, "sigmoid": 1}
 
 _KIND = {SIZE_MISMATCH: "SizeMismatch", SHAPE_MISMATCH: "ShapeMismatch", UNSUPPORTED: "Unsupported",
@@ -88,16 +89,28 @@ def _tptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
-def _dtype(t):
-    """tpt_cuda.h's code of a torch tensor's type (-1: none, refused by the library)."""
-    return {"torch.float32": DT_F32, "torch.bfloat16": DT_BF16, "torch.float16": DT_F16}.get(str(t.dtype), -1)
+class _Codes(dict):
+    """torch type -> tpt_cuda.h's code, filled in on first sight (torch is not imported here). The codes past F16
+    are the wrappers' own."""
+
+    _names = {"torch.float32": DT_F32, "torch.bfloat16": DT_BF16, "torch.float16": DT_F16, "torch.int32": _I32,
+              "torch.uint8": _U8}
+
+    def __missing__(self, dt):
+        self[dt] = self._names.get(str(dt), -1)
+        return self[dt]
 
 
-def _rows(t, cols=None):
+_CODE = _Codes()
+
+
+def _rows(t):
     """The row stride of a 2-D device tensor whose rows are contiguous."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (cols is not None and t.shape[1] != cols):
+    rows, cols = t.shape
+    s = t.stride()
+    if s[1] != 1 and cols > 1:
         raise OpError(SHAPE_MISMATCH)
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return s[0] if rows > 1 else cols
 
 
 class Weights:
@@ -449,29 +462,41 @@ class CudaBackend:
 
     # ------------------------------------------------------------ 16-bit products and experts
     def _on_device(self, *tensors):
+        dev = self.device
         for t in tensors:
-            if t is not None and (not t.is_cuda or t.device.index != self.device):
+            if t is not None and t.get_device() != dev:
                 raise OpError(INVALID)
 
     def linear_dev(self, x, w, bias, act, residual, out):
         """out[m, n] = act(x[m, k] w[n, k]^T + bias[n]) + residual[m, n], bf16 or f16 operands; ``out`` of their
         type or f32, ``residual`` of ``out``'s type (or None; it may be ``out``). Rows may be strided."""
         self._on_device(x, w, bias, residual, out)
-        if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        if x.dim() != 2 or w.dim() != 2 or out.dim() != 2:
             raise OpError(SHAPE_MISMATCH)
-        m, k = x.shape
-        n = w.shape[0]
-        if tuple(out.shape) != (m, n) or (residual is not None and tuple(residual.shape) != (m, n)):
+        (m, k), (n, kw) = x.shape, w.shape
+        ct, co = _CODE[x.dtype], _CODE[out.dtype]
+        if k != kw or out.shape != (m, n):
             raise OpError(SHAPE_MISMATCH)
-        if bias is not None and (tuple(bias.shape) != (n,) or not bias.is_contiguous()):
-            raise OpError(SHAPE_MISMATCH)
-        if w.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype) or (
-                residual is not None and residual.dtype != out.dtype):
+        if _CODE[w.dtype] != ct:
             raise OpError(UNSUPPORTED)
-        self._check(lib.tpt_cuda_linear_dev(
-            self._ctx, _dtype(x), x.data_ptr(), _rows(x), m, k, w.data_ptr(), _rows(w), n,
-            None if bias is None else bias.data_ptr(), act, None if residual is None else residual.data_ptr(),
-            0 if residual is None else _rows(residual), out.data_ptr(), _rows(out), _dtype(out)))
+        pb = pr = None
+        ldr = 0
+        if bias is not None:
+            if bias.shape != (n,) or not bias.is_contiguous():
+                raise OpError(SHAPE_MISMATCH)
+            if _CODE[bias.dtype] != ct:
+                raise OpError(UNSUPPORTED)
+            pb = bias.data_ptr()
+        if residual is not None:
+            if residual.shape != (m, n):
+                raise OpError(SHAPE_MISMATCH)
+            if _CODE[residual.dtype] != co:
+                raise OpError(UNSUPPORTED)
+            pr, ldr = residual.data_ptr(), _rows(residual)
+        st = lib.tpt_cuda_linear_dev(self._ctx, ct, x.data_ptr(), _rows(x), m, k, w.data_ptr(), _rows(w), n, pb, act,
+                                     pr, ldr, out.data_ptr(), _rows(out), co)
+        if st:
+            self._check(st)
 
     def route_experts_dev(self, logits, top_k, ids, weights, score="softmax", bias=None, groups=1, groups_kept=1,
                           group_top=1, renormalise=True, scale=1.0, mask=None):
@@ -479,46 +504,61 @@ class CudaBackend:
         f16; ids [tokens, top_k] int32 and weights [tokens, top_k] f32 are written. ``bias`` [experts] f32 orders the
         experts without entering the weights; ``mask`` [tokens] uint8, 0 for tokens that take no expert."""
         self._on_device(logits, ids, weights, bias, mask)
-        ld = _rows(logits)
+        if logits.dim() != 2:
+            raise OpError(SHAPE_MISMATCH)
         t, e = logits.shape
-        for o, dt in ((ids, "torch.int32"), (weights, "torch.float32")):
-            if str(o.dtype) != dt:
+        if _CODE[ids.dtype] != _I32 or _CODE[weights.dtype] != DT_F32:
+            raise OpError(UNSUPPORTED)
+        want = (t, top_k)
+        if ids.shape != want or weights.shape != want or not (ids.is_contiguous() and weights.is_contiguous()):
+            raise OpError(SHAPE_MISMATCH)
+        pb = pm = None
+        if bias is not None:
+            if _CODE[bias.dtype] != DT_F32:
                 raise OpError(UNSUPPORTED)
-            if tuple(o.shape) != (t, top_k) or not o.is_contiguous():
+            if bias.shape != (e,) or not bias.is_contiguous():
                 raise OpError(SHAPE_MISMATCH)
-        for o, n, dt in ((bias, e, "torch.float32"), (mask, t, "torch.uint8")):
-            if o is not None and str(o.dtype) != dt:
+            pb = bias.data_ptr()
+        if mask is not None:
+            if _CODE[mask.dtype] != _U8:
                 raise OpError(UNSUPPORTED)
-            if o is not None and (tuple(o.shape) != (n,) or not o.is_contiguous()):
+            if mask.shape != (t,) or not mask.is_contiguous():
                 raise OpError(SHAPE_MISMATCH)
+            pm = mask.data_ptr()
         if score not in _SCORES:
             raise OpError(INVALID)
-        self._check(lib.tpt_cuda_route_experts_dev(
-            self._ctx, logits.data_ptr(), _dtype(logits), ld, t, e, _SCORES[score],
-            None if bias is None else bias.data_ptr(), groups, groups_kept, group_top, top_k, int(renormalise),
-            scale, None if mask is None else mask.data_ptr(), ids.data_ptr(), weights.data_ptr()))
+        st = lib.tpt_cuda_route_experts_dev(self._ctx, logits.data_ptr(), _CODE[logits.dtype], _rows(logits), t, e,
+                                            _SCORES[score], pb, groups, groups_kept, group_top, top_k,
+                                            int(renormalise), scale, pm, ids.data_ptr(), weights.data_ptr())
+        if st:
+            self._check(st)
 
     def experts_mlp_dev(self, x, ids, weights, w_in, w_out, act, gated, residual, out):
         """The chosen experts' feed-forward layers, weighted and summed (tpt_cuda_experts_mlp_dev): x [tokens, d],
         ids / weights [tokens, top_k], w_in [experts, f or 2 f, d], w_out [experts, d, f], bf16 or f16 throughout;
         ``residual`` is added (None: nothing; it may be ``out``)."""
         self._on_device(x, ids, weights, w_in, w_out, residual, out)
-        if x.dim() != 2 or ids.dim() != 2 or w_in.dim() != 3 or w_out.dim() != 3:
+        if x.dim() != 2 or ids.dim() != 2 or w_in.dim() != 3 or w_out.dim() != 3 or out.dim() != 2:
             raise OpError(SHAPE_MISMATCH)
-        (t, d), k = x.shape, ids.shape[1]
-        e, f = w_out.shape[0], w_out.shape[2]
-        if tuple(w_out.shape) != (e, d, f) or tuple(w_in.shape) != (e, 2 * f if gated else f, d):
-            raise OpError(SHAPE_MISMATCH)
-        if tuple(ids.shape) != (t, k) or tuple(weights.shape) != (t, k) or tuple(out.shape) != (t, d) or (
-                residual is not None and tuple(residual.shape) != (t, d)):
+        (t, d), k, (e, wd, f) = x.shape, ids.shape[1], w_out.shape
+        if wd != d or w_in.shape != (e, 2 * f if gated else f, d) or ids.shape != (t, k) or (
+                weights.shape != (t, k) or out.shape != (t, d)):
             raise OpError(SHAPE_MISMATCH)
         if not (ids.is_contiguous() and weights.is_contiguous() and w_in.is_contiguous() and w_out.is_contiguous()):
             raise OpError(SHAPE_MISMATCH)
-        if str(ids.dtype) != "torch.int32" or str(weights.dtype) != "torch.float32" or any(
-                o is not None and o.dtype != x.dtype for o in (w_in, w_out, residual, out)):
+        ct = _CODE[x.dtype]
+        if _CODE[ids.dtype] != _I32 or _CODE[weights.dtype] != DT_F32 or not (
+                ct == _CODE[w_in.dtype] == _CODE[w_out.dtype] == _CODE[out.dtype]):
             raise OpError(UNSUPPORTED)
-        self._check(lib.tpt_cuda_experts_mlp_dev(
-            self._ctx, _dtype(x), x.data_ptr(), _rows(x), t, d, ids.data_ptr(), weights.data_ptr(), k,
-            w_in.data_ptr(), w_out.data_ptr(), e, f, act, int(gated),
-            None if residual is None else residual.data_ptr(), 0 if residual is None else _rows(residual),
-            out.data_ptr(), _rows(out)))
+        pr, ldr = None, 0
+        if residual is not None:
+            if residual.shape != (t, d):
+                raise OpError(SHAPE_MISMATCH)
+            if _CODE[residual.dtype] != ct:
+                raise OpError(UNSUPPORTED)
+            pr, ldr = residual.data_ptr(), _rows(residual)
+        st = lib.tpt_cuda_experts_mlp_dev(self._ctx, ct, x.data_ptr(), _rows(x), t, d, ids.data_ptr(),
+                                          weights.data_ptr(), k, w_in.data_ptr(), w_out.data_ptr(), e, f, act,
+                                          int(gated), pr, ldr, out.data_ptr(), _rows(out))
+        if st:
+            self._check(st)

@@ -11,6 +11,8 @@
 // The order of an expert's slots has no influence on the results: a slot's
 // sums do not depend on its neighbours, and the sum over a token's experts
 // runs in the order of its choices.
+#include <type_traits>
+
 #include "gemm16.cuh"
 
 namespace tpt {
@@ -26,138 +28,158 @@ __device__ __forceinline__ unsigned order_key(float v) {
     return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-// One warp per token; lane l holds experts l * V .. l * V + V - 1, so that of
-// equal values the lowest lane's lowest one is the lowest expert.
+// V consecutive logits; vec: as 16-, 8- or 4-byte words
+template <typename T, int V>
+__device__ __forceinline__ void load_logits(const T *p, bool vec, int n, float (&s)[V]) {
+    constexpr int B = V * sizeof(T) >= 16 ? 16 : V * sizeof(T);  // bytes of a word
+    constexpr int N = B / sizeof(T);
+    if (B >= 4 && vec) {
+        using W = typename std::conditional<B == 16, uint4, typename std::conditional<B == 8, uint2, uint32_t>::type>::type;
+        if (n > 0) {
+#pragma unroll
+            for (int i = 0; i < V; i += N) {
+                union {
+                    W w;
+                    T t[N];
+                } u;
+                u.w = *reinterpret_cast<const W *>(p + i);
+#pragma unroll
+                for (int j = 0; j < N; j++) s[i + j] = to_f32(u.t[j]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++) s[i] = -INFINITY;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) s[i] = i < n ? to_f32(p[i]) : -INFINITY;
+    }
+}
+// the score of one logit: the largest logit itself by comparison, so that its
+// term is 1 for +inf too
+__device__ __forceinline__ float route_score(float l, bool softmax, float top, float rsum) {
+    if (l == -INFINITY) return 0.0f;
+    return softmax ? (l == top ? 1.0f : expf(l - top)) * rsum : __frcp_rn(1.0f + expf(-l));
+}
+
+// One warp per token. Each group has `lanes` (a power of two) neighbouring
+// lanes and each of them V of its experts in order, so a group's best values
+// meet in log2(lanes) exchanges, and of equal values the lowest lane's lowest
+// one is the lowest expert. The chosen experts come out one per round: the
+// warp's largest key, its first lane, that lane's next best. What it does is
+// bound by instructions, not by the 4 E bytes it reads.
 template <typename T, int V>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32)
-    k_route_experts(const T *__restrict__ logits, size_t ld, int tokens, int experts, int score,
-                    const float *__restrict__ bias, int groups, int groups_kept, int group_top, int top_k,
-                    int renormalise, float scale, const uint8_t *__restrict__ mask, int *__restrict__ ids,
+    k_route_experts(const T *__restrict__ logits, size_t ld, int tokens, int experts, int softmax,
+                    const float *__restrict__ bias, int groups, int groups_kept, int group_top, int lanes, int vec,
+                    int top_k, int renormalise, float scale, const uint8_t *__restrict__ mask, int *__restrict__ ids,
                     float *__restrict__ weights) {
     pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31;
     const int t = blockIdx.x * ROUTE_WARPS + (threadIdx.x >> 5);
     if (t >= tokens) return;
-    int *my_ids = ids + (size_t)t * top_k;
-    float *my_w = weights + (size_t)t * top_k;
-    if (mask && !mask[t]) {
-        for (int j = lane; j < top_k; j += 32) {
-            my_ids[j] = -1;
-            my_w[j] = 0.0f;
-        }
-        return;
-    }
-    const float NEG = -INFINITY;
-    const T *row = logits + (size_t)t * ld;
-    float s[V], c[V];
-    float top = NEG;
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-        const int e = lane * V + i;
-        const float l = e < experts ? to_f32(row[e]) : NEG;
-        s[i] = l > NEG ? l : NEG;  // NaN: an expert that cannot be chosen
-        top = fmaxf(top, s[i]);
-    }
-    if (score == TPT_SCORE_SOFTMAX) {
-        top = warp_max(top);
-        float sum = 0.0f;
+    int id_mine = -1;  // lane j keeps choice j
+    float w_mine = 0.0f;
+    if (!mask || mask[t]) {
+        const float NEG = -INFINITY;
+        const int per = experts / groups, q = lane / lanes, at0 = (lane & (lanes - 1)) * V;
+        const int n = q < groups ? min(V, per - at0) : 0;  // this lane's experts (none: n <= 0)
+        const int e0 = q * per + at0;
+        const T *row = logits + (size_t)t * ld;
+        float c[V];
+        load_logits<T, V>(row + e0, vec, n, c);
+        float top = NEG, rsum = 1.0f;
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            c[i] = s[i];
-            // the largest logit itself by comparison: its term is 1 for +inf too
-            s[i] = s[i] == NEG ? 0.0f : s[i] == top ? 1.0f : expf(s[i] - top);
-            sum += s[i];
+            c[i] = c[i] > NEG ? c[i] : NEG;  // NaN: an expert that cannot be chosen
+            top = fmaxf(top, c[i]);
         }
-        sum = warp_sum(sum);
+        if (softmax) {
+            top = warp_max(top);
+            float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; i++) s[i] = sum > 0.0f ? s[i] / sum : 0.0f;
-    } else {
+            for (int i = 0; i < V; i++) {
+                const float s = route_score(c[i], true, top, 1.0f);
+                sum += s;
+                c[i] = c[i] == NEG ? NEG : s;
+            }
+            sum = warp_sum(sum);
+            rsum = sum > 0.0f ? __frcp_rn(sum) : 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            c[i] = s[i];
-            s[i] = s[i] == NEG ? 0.0f : 1.0f / (1.0f + expf(-s[i]));
+            for (int i = 0; i < V; i++) c[i] = c[i] == NEG ? NEG : c[i] * rsum;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++) c[i] = c[i] == NEG ? NEG : route_score(c[i], false, 0.0f, 1.0f);
         }
-    }
+        if (bias) {
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        const int e = lane * V + i;
-        const float b = c[i] == NEG ? NEG : bias ? s[i] + bias[e] : s[i];
-        c[i] = b > NEG ? b : NEG;  // a NaN or -inf bias switches the expert off
-    }
-    if (groups > 1) {
-        // lane q's verdict on group q; each group's best one or two values by
-        // warp maxima over the lanes' members
-        const int per = experts / groups;
-        float mine = NEG;
-        for (int q = 0; q < groups; q++) {
+            for (int i = 0; i < V; i++) {
+                const float b = c[i] == NEG ? NEG : c[i] + (i < n ? __ldg(bias + e0 + i) : 0.0f);
+                c[i] = b > NEG ? b : NEG;  // a NaN or -inf bias switches the expert off
+            }
+        }
+        if (groups > 1) {
             float b1 = NEG, b2 = NEG;
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const int e = lane * V + i;
-                const float v = e >= q * per && e < (q + 1) * per ? c[i] : NEG;
-                if (v > b1) {
-                    b2 = b1;
-                    b1 = v;
-                } else {
-                    b2 = fmaxf(b2, v);
-                }
+                b2 = fmaxf(b2, fminf(b1, c[i]));
+                b1 = fmaxf(b1, c[i]);
             }
-            const float m1 = warp_max(b1);
-            if (group_top == 2 && m1 > NEG) {
-                const int owner = __ffs(__ballot_sync(0xffffffffu, b1 == m1)) - 1;
-                const float m2 = warp_max(lane == owner ? b2 : b1);
-                b1 = m2 > NEG ? m1 + m2 : m1;
-            } else {
-                b1 = m1;
+            for (int o = 1; o < lanes; o <<= 1) {
+                const float p1 = __shfl_xor_sync(0xffffffffu, b1, o), p2 = __shfl_xor_sync(0xffffffffu, b2, o);
+                b2 = fmaxf(fminf(b1, p1), fmaxf(b2, p2));
+                b1 = fmaxf(b1, p1);
             }
-            if (lane == q) mine = b1;
-        }
-        unsigned kept = 0;
-        for (int r = 0; r < groups_kept; r++) {
-            const unsigned key = lane < groups && !(kept >> lane & 1) ? order_key(mine + 0.0f) : 0u;
-            const unsigned best = __reduce_max_sync(0xffffffffu, key);
-            kept |= 1u << (__ffs(__ballot_sync(0xffffffffu, key == best && lane < groups && !(kept >> lane & 1))) - 1);
-        }
+            const float mine = group_top == 2 && b2 > NEG ? b1 + b2 : b1;
+            int better = 0;
+            for (int g = 0; g < groups; g++) {
+                const float o = __shfl_sync(0xffffffffu, mine, g * lanes);
+                better += o > mine || (o == mine && g < q) ? 1 : 0;
+            }
+            if (better >= groups_kept) {
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            const int e = lane * V + i;
-            if (e < experts && !(kept >> (e / per) & 1)) c[i] = NEG;
+                for (int i = 0; i < V; i++) c[i] = NEG;
+            }
         }
-    }
-    float w_mine = 0.0f, sum = 0.0f;  // lane j keeps choice j
-    int id_mine = -1;
-    for (int j = 0; j < top_k; j++) {
-        float b = NEG, sv = 0.0f;
+        float b = NEG;
         int at = 0;
 #pragma unroll
         for (int i = 0; i < V; i++)
             if (c[i] > b) {
                 b = c[i];
-                sv = s[i];
                 at = i;
             }
-        const unsigned key = order_key(b + 0.0f);  // -0 counts as 0
-        const unsigned best = __reduce_max_sync(0xffffffffu, key);
-        if (best == order_key(NEG)) break;  // no expert is left
-        const int owner = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1;
-        const int e = __shfl_sync(0xffffffffu, lane * V + at, owner);
-        const float w = __shfl_sync(0xffffffffu, sv, owner);
-        sum += w;
-        if (lane == j) {
-            id_mine = e;
-            w_mine = w;
-        }
-        if (lane == owner) {
+        for (int j = 0; j < top_k; j++) {
+            const unsigned key = order_key(b + 0.0f);  // -0 counts as 0
+            const unsigned best = __reduce_max_sync(0xffffffffu, key);
+            if (best == order_key(NEG)) break;  // no expert is left
+            const int owner = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1;
+            const int e = __shfl_sync(0xffffffffu, e0 + at, owner);
+            if (lane == j) id_mine = e;
+            if (lane == owner) {
+                const int gone = at;
+                b = NEG;
 #pragma unroll
-            for (int i = 0; i < V; i++)
-                if (i == at) c[i] = NEG;
+                for (int i = 0; i < V; i++) {
+                    if (i == gone) c[i] = NEG;
+                    if (c[i] > b) {
+                        b = c[i];
+                        at = i;
+                    }
+                }
+            }
         }
+        if (id_mine >= 0) w_mine = route_score(to_f32(row[id_mine]), softmax, top, rsum);
+        if (renormalise) {
+            const float sum = warp_sum(w_mine);
+            w_mine = sum > 0.0f ? w_mine / sum : 0.0f;
+        }
+        w_mine *= scale;
     }
-    if (renormalise) w_mine = sum > 0.0f ? w_mine / sum : 0.0f;
     if (lane < top_k) {
-        my_ids[lane] = id_mine;
-        my_w[lane] = w_mine * scale;
+        ids[(size_t)t * top_k + lane] = id_mine;
+        weights[(size_t)t * top_k + lane] = w_mine;
     }
 }
 
@@ -166,22 +188,33 @@ void launch_route(tpt_cuda_ctx *ctx, const void *logits, size_t ld, int tokens, 
                   const float *bias, int groups, int groups_kept, int group_top, int top_k, int renormalise,
                   float scale, const uint8_t *mask, int *ids, float *weights) {
     const dim3 grid((tokens + ROUTE_WARPS - 1) / ROUTE_WARPS);
+    int lanes = 32;
+    while (lanes * groups > 32) lanes /= 2;
+    const int per = experts / groups, need = (per + lanes - 1) / lanes;
+    int v = 1;
+    while (v < need) v *= 2;
+    const size_t word = v * sizeof(T) < 16 ? v * sizeof(T) : 16;
+    const bool vec = per % v == 0 && ((uintptr_t)logits % word) == 0 && (tokens == 1 || ld * sizeof(T) % word == 0);
     auto go = [&](auto kern) {
-        launch_pdl(kern, grid, ROUTE_WARPS * 32, 0, ctx->stream, (const T *)logits, ld, tokens, experts, score, bias,
-                   groups, groups_kept, group_top, top_k, renormalise, scale, mask, ids, weights);
+        launch_pdl(kern, grid, ROUTE_WARPS * 32, 0, ctx->stream, (const T *)logits, ld, tokens, experts,
+                   score == TPT_SCORE_SOFTMAX, bias, groups, groups_kept, group_top, lanes, vec, top_k, renormalise,
+                   scale, mask, ids, weights);
     };
-    if (experts <= 32)
+    // groups <= 32 and experts <= 1024: at most 64 experts a lane (17 groups of 60)
+    if (v == 1)
         go(k_route_experts<T, 1>);
-    else if (experts <= 64)
+    else if (v == 2)
         go(k_route_experts<T, 2>);
-    else if (experts <= 128)
+    else if (v == 4)
         go(k_route_experts<T, 4>);
-    else if (experts <= 256)
+    else if (v == 8)
         go(k_route_experts<T, 8>);
-    else if (experts <= 512)
+    else if (v == 16)
         go(k_route_experts<T, 16>);
-    else
+    else if (v == 32)
         go(k_route_experts<T, 32>);
+    else
+        go(k_route_experts<T, 64>);
 }
 
 // ------------------------------------------------------------------ the slots
