@@ -24,6 +24,8 @@ ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
 DT_F32, DT_BF16, DT_F16 = 0, 2, 3
 _I32, _U8 = 100, 101
 _SCORES = {"softmax": 0, "sigmoid": 1}
+_linear, _route, _experts = (lib.tpt_cuda_linear_dev, lib.tpt_cuda_route_experts_dev,
+                            lib.tpt_cuda_experts_mlp_dev)
 
 _KIND = {SIZE_MISMATCH: "SizeMismatch", SHAPE_MISMATCH: "ShapeMismatch", UNSUPPORTED: "Unsupported",
          INVALID: "Invalid"}
@@ -107,10 +109,10 @@ _CODE = _Codes()
 def _rows(t):
     """The row stride of a 2-D device tensor whose rows are contiguous."""
     rows, cols = t.shape
-    s = t.stride()
-    if s[1] != 1 and cols > 1:
+    r, c = t.stride()
+    if c != 1 and cols > 1:
         raise OpError(SHAPE_MISMATCH)
-    return s[0] if rows > 1 else cols
+    return r if rows > 1 else cols
 
 
 class Weights:
@@ -461,40 +463,43 @@ class CudaBackend:
         self._check(lib.tpt_cuda_matmul_dev(self._ctx, _tptr(a), m, k, _tptr(b), n, _tptr(out)))
 
     # ------------------------------------------------------------ 16-bit products and experts
-    def _on_device(self, *tensors):
-        dev = self.device
-        for t in tensors:
-            if t is not None and t.get_device() != dev:
-                raise OpError(INVALID)
-
+    # Decoding calls these once per layer and token, so their checks are written for the time they take: a
+    # contiguous tensor's strides are not asked for, and shapes are taken apart once.
     def linear_dev(self, x, w, bias, act, residual, out):
         """out[m, n] = act(x[m, k] w[n, k]^T + bias[n]) + residual[m, n], bf16 or f16 operands; ``out`` of their
         type or f32, ``residual`` of ``out``'s type (or None; it may be ``out``). Rows may be strided."""
-        self._on_device(x, w, bias, residual, out)
-        if x.dim() != 2 or w.dim() != 2 or out.dim() != 2:
-            raise OpError(SHAPE_MISMATCH)
-        (m, k), (n, kw) = x.shape, w.shape
-        ct, co = _CODE[x.dtype], _CODE[out.dtype]
-        if k != kw or out.shape != (m, n):
-            raise OpError(SHAPE_MISMATCH)
-        if _CODE[w.dtype] != ct:
+        dev, ty, oty = self.device, x.dtype, out.dtype
+        if x.get_device() != dev or w.get_device() != dev or out.get_device() != dev:
+            raise OpError(INVALID)
+        if w.dtype != ty:
             raise OpError(UNSUPPORTED)
+        try:
+            (m, k), (n, kw), (om, on) = x.shape, w.shape, out.shape
+        except ValueError:
+            raise OpError(SHAPE_MISMATCH) from None
+        if k != kw or om != m or on != n:
+            raise OpError(SHAPE_MISMATCH)
         pb = pr = None
         ldr = 0
         if bias is not None:
+            if bias.get_device() != dev:
+                raise OpError(INVALID)
             if bias.shape != (n,) or not bias.is_contiguous():
                 raise OpError(SHAPE_MISMATCH)
-            if _CODE[bias.dtype] != ct:
+            if bias.dtype != ty:
                 raise OpError(UNSUPPORTED)
             pb = bias.data_ptr()
         if residual is not None:
+            if residual.get_device() != dev:
+                raise OpError(INVALID)
             if residual.shape != (m, n):
                 raise OpError(SHAPE_MISMATCH)
-            if _CODE[residual.dtype] != co:
+            if residual.dtype != oty:
                 raise OpError(UNSUPPORTED)
-            pr, ldr = residual.data_ptr(), _rows(residual)
-        st = lib.tpt_cuda_linear_dev(self._ctx, ct, x.data_ptr(), _rows(x), m, k, w.data_ptr(), _rows(w), n, pb, act,
-                                     pr, ldr, out.data_ptr(), _rows(out), co)
+            pr, ldr = residual.data_ptr(), n if residual.is_contiguous() else _rows(residual)
+        st = _linear(self._ctx, _CODE[ty], x.data_ptr(), k if x.is_contiguous() else _rows(x), m, k, w.data_ptr(),
+                     k if w.is_contiguous() else _rows(w), n, pb, act, pr, ldr, out.data_ptr(),
+                     n if out.is_contiguous() else _rows(out), _CODE[oty])
         if st:
             self._check(st)
 
@@ -503,23 +508,29 @@ class CudaBackend:
         """Chooses each token's ``top_k`` experts (tpt_cuda_route_experts_dev): logits [tokens, experts] f32, bf16 or
         f16; ids [tokens, top_k] int32 and weights [tokens, top_k] f32 are written. ``bias`` [experts] f32 orders the
         experts without entering the weights; ``mask`` [tokens] uint8, 0 for tokens that take no expert."""
-        self._on_device(logits, ids, weights, bias, mask)
-        if logits.dim() != 2:
-            raise OpError(SHAPE_MISMATCH)
-        t, e = logits.shape
+        dev = self.device
+        if logits.get_device() != dev or ids.get_device() != dev or weights.get_device() != dev:
+            raise OpError(INVALID)
         if _CODE[ids.dtype] != _I32 or _CODE[weights.dtype] != DT_F32:
             raise OpError(UNSUPPORTED)
-        want = (t, top_k)
-        if ids.shape != want or weights.shape != want or not (ids.is_contiguous() and weights.is_contiguous()):
+        try:
+            (t, e), (it, ik), (wt, wk) = logits.shape, ids.shape, weights.shape
+        except ValueError:
+            raise OpError(SHAPE_MISMATCH) from None
+        if it != t or wt != t or ik != top_k or wk != top_k or not (ids.is_contiguous() and weights.is_contiguous()):
             raise OpError(SHAPE_MISMATCH)
         pb = pm = None
         if bias is not None:
+            if bias.get_device() != dev:
+                raise OpError(INVALID)
             if _CODE[bias.dtype] != DT_F32:
                 raise OpError(UNSUPPORTED)
             if bias.shape != (e,) or not bias.is_contiguous():
                 raise OpError(SHAPE_MISMATCH)
             pb = bias.data_ptr()
         if mask is not None:
+            if mask.get_device() != dev:
+                raise OpError(INVALID)
             if _CODE[mask.dtype] != _U8:
                 raise OpError(UNSUPPORTED)
             if mask.shape != (t,) or not mask.is_contiguous():
@@ -527,9 +538,9 @@ class CudaBackend:
             pm = mask.data_ptr()
         if score not in _SCORES:
             raise OpError(INVALID)
-        st = lib.tpt_cuda_route_experts_dev(self._ctx, logits.data_ptr(), _CODE[logits.dtype], _rows(logits), t, e,
-                                            _SCORES[score], pb, groups, groups_kept, group_top, top_k,
-                                            int(renormalise), scale, pm, ids.data_ptr(), weights.data_ptr())
+        st = _route(self._ctx, logits.data_ptr(), _CODE[logits.dtype],
+                    e if logits.is_contiguous() else _rows(logits), t, e, _SCORES[score], pb, groups, groups_kept,
+                    group_top, top_k, 1 if renormalise else 0, scale, pm, ids.data_ptr(), weights.data_ptr())
         if st:
             self._check(st)
 
@@ -537,28 +548,34 @@ class CudaBackend:
         """The chosen experts' feed-forward layers, weighted and summed (tpt_cuda_experts_mlp_dev): x [tokens, d],
         ids / weights [tokens, top_k], w_in [experts, f or 2 f, d], w_out [experts, d, f], bf16 or f16 throughout;
         ``residual`` is added (None: nothing; it may be ``out``)."""
-        self._on_device(x, ids, weights, w_in, w_out, residual, out)
-        if x.dim() != 2 or ids.dim() != 2 or w_in.dim() != 3 or w_out.dim() != 3 or out.dim() != 2:
-            raise OpError(SHAPE_MISMATCH)
-        (t, d), k, (e, wd, f) = x.shape, ids.shape[1], w_out.shape
-        if wd != d or w_in.shape != (e, 2 * f if gated else f, d) or ids.shape != (t, k) or (
-                weights.shape != (t, k) or out.shape != (t, d)):
+        dev, ty = self.device, x.dtype
+        for v in (x, ids, weights, w_in, w_out, out):
+            if v.get_device() != dev:
+                raise OpError(INVALID)
+        try:
+            (t, d), (it, k), (wt, wk), (e, wd, f), (ie, iu, idim), (ot, od) = (
+                x.shape, ids.shape, weights.shape, w_out.shape, w_in.shape, out.shape)
+        except ValueError:
+            raise OpError(SHAPE_MISMATCH) from None
+        if (it != t or wt != t or ot != t or wk != k or wd != d or idim != d or od != d or ie != e or
+                iu != (2 * f if gated else f)):
             raise OpError(SHAPE_MISMATCH)
         if not (ids.is_contiguous() and weights.is_contiguous() and w_in.is_contiguous() and w_out.is_contiguous()):
             raise OpError(SHAPE_MISMATCH)
-        ct = _CODE[x.dtype]
-        if _CODE[ids.dtype] != _I32 or _CODE[weights.dtype] != DT_F32 or not (
-                ct == _CODE[w_in.dtype] == _CODE[w_out.dtype] == _CODE[out.dtype]):
+        if (_CODE[ids.dtype] != _I32 or _CODE[weights.dtype] != DT_F32 or w_in.dtype != ty or w_out.dtype != ty or
+                out.dtype != ty):
             raise OpError(UNSUPPORTED)
         pr, ldr = None, 0
         if residual is not None:
+            if residual.get_device() != dev:
+                raise OpError(INVALID)
             if residual.shape != (t, d):
                 raise OpError(SHAPE_MISMATCH)
-            if _CODE[residual.dtype] != ct:
+            if residual.dtype != ty:
                 raise OpError(UNSUPPORTED)
-            pr, ldr = residual.data_ptr(), _rows(residual)
-        st = lib.tpt_cuda_experts_mlp_dev(self._ctx, ct, x.data_ptr(), _rows(x), t, d, ids.data_ptr(),
-                                          weights.data_ptr(), k, w_in.data_ptr(), w_out.data_ptr(), e, f, act,
-                                          int(gated), pr, ldr, out.data_ptr(), _rows(out))
+            pr, ldr = residual.data_ptr(), d if residual.is_contiguous() else _rows(residual)
+        st = _experts(self._ctx, _CODE[ty], x.data_ptr(), d if x.is_contiguous() else _rows(x), t, d, ids.data_ptr(),
+                      weights.data_ptr(), k, w_in.data_ptr(), w_out.data_ptr(), e, f, act, 1 if gated else 0, pr, ldr,
+                      out.data_ptr(), d if out.is_contiguous() else _rows(out))
         if st:
             self._check(st)
