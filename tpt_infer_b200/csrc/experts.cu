@@ -423,6 +423,41 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
                 bool gated, const T *residual, size_t ldr, T *y, size_t ldy) {
     auto up8 = [](size_t v) { return (v + 7) / 8 * 8; };
     const size_t ldh = up8(f), lds = up8(d), ldp = (d + 3) / 4 * 4;  // rows start on 16 bytes
+    if (tokens <= 8 && tokens * top_k <= STREAM_PAIRS && stream_x_bytes(tokens, d) <= STREAM_X_BYTES &&
+        stream_x_bytes(tokens * top_k, f) <= STREAM_X_BYTES) {
+        const size_t tiles = tokens * top_k < experts ? tokens * top_k : experts;
+        int st = ensure_ws(ctx, tiles * 8 * ldh * 2);
+        if (st) return st;
+        Gemm16 g;
+        g.x = x;
+        g.ldx = ldx;
+        g.x_rows = (int)tokens;
+        g.w = w_in;
+        g.ldw = d;
+        g.w_expert = (gated ? 2 : 1) * f * d;
+        g.n = (int)f;
+        g.k = (int)d;
+        g.experts = (int)experts;
+        g.act = act;
+        g.gated = gated;
+        g.y = ctx->ws;
+        g.ldy = ldh;
+        Gemm16 o;
+        o.x = ctx->ws;
+        o.ldx = ldh;
+        o.x_rows = 8;
+        o.w = w_out;
+        o.ldw = f;
+        o.w_expert = d * f;
+        o.n = (int)d;
+        o.k = (int)f;
+        o.experts = (int)experts;
+        o.residual = residual;
+        o.ldr = ldr;
+        o.y = y;
+        o.ldy = ldy;
+        return launch_experts_stream(ctx, dtype, g, o, ids, weights, (int)(tokens * top_k), (int)top_k);
+    }
     // Tokens per tile of the products: what an expert gets on average, up to the
     // pair kernel's 256 columns.
     const size_t mean = (tokens * top_k + experts - 1) / experts;

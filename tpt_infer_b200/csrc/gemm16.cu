@@ -61,6 +61,8 @@ int tpt_cuda_linear_dev(tpt_cuda_ctx *ctx, int dtype, const void *x, size_t ldx,
     g.y = y;
     g.ldy = ldy;
     g.y_f32 = y_dtype == TPT_DT_F32;
+    if (k > 0 && m <= STREAM_TOKENS && stream_x_bytes(m, k) <= STREAM_X_BYTES)
+        return launch_gemm16_stream(ctx, dtype, g);
     // TMA reads rows that start on 16 bytes; others are copied to the workspace
     // first (k = 0 becomes eight zero products).
     const size_t k8 = k ? (k + 7) / 8 * 8 : 8;

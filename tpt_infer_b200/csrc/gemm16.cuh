@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "tc_common.cuh"
 
 namespace tpt {
@@ -47,6 +49,19 @@ struct Gemm16 {
 // Device enqueue; dtype TPT_DT_BF16 or TPT_DT_F16, k > 0. The operands' rows
 // must pass rows16_ok (the copies below make them).
 int launch_gemm16(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g);
+
+// The kernels of a few tokens, for operands of any alignment: a dense product of
+// up to STREAM_TOKENS rows, and both of the experts' products of up to
+// STREAM_PAIRS (token, choice) pairs of up to 8 tokens. `in` reads the tokens'
+// rows and writes [tile][8][ldy], one tile per distinct expert; `out` reads
+// those and writes the tokens' weighted sums.
+// The tokens' rows have to fit STREAM_X_BYTES of shared memory.
+constexpr int STREAM_TOKENS = 16, STREAM_PAIRS = 32;
+constexpr size_t STREAM_X_BYTES = 80 * 1024;
+inline size_t stream_x_bytes(size_t rows, size_t k) { return rows * ((k + 63) / 64 * 128 + 16); }
+int launch_gemm16_stream(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g);
+int launch_experts_stream(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &in, const Gemm16 &out, const int *ids,
+                          const float *weights, int pairs, int top_k);
 
 // Whether TMA can read `rows` rows of 16-bit values ld apart: base and rows on
 // 16 bytes.

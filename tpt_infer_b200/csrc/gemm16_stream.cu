@@ -1,0 +1,389 @@
+// gemm16_stream.cu -- the 16-bit products of a few tokens, bound by the stream
+// of the weights: a decoding step's linear layers and its tokens' experts.
+//
+// The weights go from memory to registers in 128-bit loads, several per thread
+// in flight, and straight into mma.sync m16n8k16 as the A operand (16 weight
+// rows; the tokens are the 8 columns). The k order within 32 values is permuted
+// the same way in both operands, so that a thread's 16 bytes of a row are its
+// fragments of two MMAs; the tokens' rows wait in shared memory. Every block
+// takes an equal range of weight rows, so the SMs' shares of the stream differ
+// by one row at most; its eight warps split k (and, summing over experts, the
+// experts), and their partial sums meet in shared memory in a fixed order.
+//
+// Measured against the tcgen05 split kernel at 1 x 4096 x 4096 (33.5 MB, 5.1 us
+// at the copy rate): there a single SM draws ~50 GB/s through TMA boxes of
+// 128-byte lines, and 256 tiles over 148 SMs leave some with twice the work.
+#include "gemm16.cuh"
+
+namespace tpt {
+namespace {
+
+constexpr int ST_WARPS = 8;
+constexpr int ST_T = ST_WARPS * 32;
+constexpr int ST_ROWS = 16;   // weight rows of one MMA
+constexpr int ST_CHUNK = 64;  // k values of one step of a warp
+
+struct StreamArgs {
+    const void *x;
+    size_t ldx;
+    int tokens;
+    const void *w;
+    size_t ldw, w_expert;
+    int n, k;
+    // grouped: the distinct experts of `pairs` ids take one tile each
+    const int *ids;
+    const float *weights;
+    int pairs, top_k, experts;
+    const void *bias;
+    int act;
+    const void *residual;
+    size_t ldr;
+    void *y;
+    size_t ldy;
+    unsigned *gflags;
+};
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Eight 16-bit values from p, of which the first n exist (the rest are 0): one
+// 128-bit load, or by single values where rows do not start on 16 bytes.
+// STREAM: read once, not kept in L1.
+template <bool AL16, bool STREAM>
+__device__ __forceinline__ uint4 load8(const uint16_t *p, int n) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if constexpr (AL16) {
+        if (n > 0) {  // n is 8 or none: k is a multiple of 8
+            if constexpr (STREAM)
+                asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                             : "l"(p));
+            else
+                v = *reinterpret_cast<const uint4 *>(p);
+        }
+    } else {
+        uint32_t e[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) e[i] = i < n ? (uint32_t)p[i] : 0u;
+        v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+    }
+    return v;
+}
+
+// GATED: y = act(W x) * (W2 x). SUM: y[token] = sum over the experts of
+// weight * W_e x_e, x the tiles' rows [tile][token]; otherwise each tile's
+// products go to y's rows [tile][token] (dense: one tile). NC: tokens / 8.
+template <typename T, typename TY, bool GATED, bool SUM, bool AL16, int NC>
+__global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant__ StreamArgs a) {
+    constexpr int H = GATED ? 2 : 1;
+    constexpr int DEPTH = GATED ? 2 : 4;  // steps in flight: 16 loads of 16 bytes a thread
+    constexpr int COLS = 8 * NC;
+    __shared__ float red[2][ST_WARPS][H][ST_ROWS][COLS];
+    __shared__ int tile_expert[32];
+    __shared__ float tile_w[SUM ? 32 : 1][8];
+    __shared__ int tile_used[SUM ? 32 : 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    __shared__ int slot_row[SUM ? 32 : 1];  // the staged rows: (tile * 8 + token) of each
+    __shared__ int tile_slot[SUM ? 32 : 1];  // a tile's first
+    extern __shared__ __align__(16) uint8_t xs[];
+    const uint16_t *w = static_cast<const uint16_t *>(a.w);
+    const uint16_t *x = static_cast<const uint16_t *>(a.x);
+    if (AL16 && !a.ids) {
+        // a dense layer's rows start towards the L2 while the kernel before it ends
+        const int r0 = (int)((long long)a.n * blockIdx.x / gridDim.x), r1 = (int)((long long)a.n * (blockIdx.x + 1) / gridDim.x);
+        for (int r = r0 + (int)threadIdx.x; r < r1; r += ST_T)
+            prefetch_l2_bulk(w + (size_t)r * a.ldw, (uint32_t)a.k * 2);
+    }
+    pdl_wait();
+    pdl_trigger();
+    int n_tiles = 1, x_rows = a.tokens;
+    if (a.ids) {
+        // the distinct experts, in the order of their first choice (every warp alike)
+        const int id = lane < a.pairs ? __ldcg(a.ids + lane) : -1;
+        const bool valid = id >= 0 && id < a.experts;
+        if (warp == 0 && id >= a.experts) atomicOr(a.gflags + TPT_FLAG_CHECK, 1u);
+        const unsigned same = __match_any_sync(0xffffffffu, valid ? id : -1 - lane);
+        const bool first = valid && __ffs(same) - 1 == lane;
+        const unsigned firsts = __ballot_sync(0xffffffffu, first);
+        n_tiles = __popc(firsts);
+        const int tile = __popc(firsts & ((1u << lane) - 1));
+        if (warp == 0 && first) tile_expert[tile] = id;
+        if (SUM) {
+            int used = 0;
+            if (first)
+                for (unsigned m = same; m; m &= m - 1) used |= 1 << ((__ffs(m) - 1) / a.top_k);
+            int end = __popc(used);  // inclusive sum over the tiles' rows
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, end, o);
+                if (lane >= o) end += v;
+            }
+            x_rows = __shfl_sync(0xffffffffu, end, 31);
+            if (warp == 0 && first) {
+                // a token that chose the expert twice takes it once, with both weights
+                for (int i = 0; i < 8; i++) tile_w[tile][i] = 0.0f;
+                for (unsigned m = same; m; m &= m - 1) {
+                    const int p = __ffs(m) - 1;
+                    tile_w[tile][p / a.top_k] += a.weights[p];
+                }
+                tile_used[tile] = used;
+                int at = end - __popc(used);
+                tile_slot[tile] = at;
+                for (int m = used; m; m &= m - 1) slot_row[at++] = tile * 8 + __ffs(m) - 1;
+            }
+        }
+        __syncthreads();
+    }
+    const int kch = (a.k + ST_CHUNK - 1) / ST_CHUNK;  // steps of one product
+    // the tokens' rows, zero past k; 16 bytes more than a multiple of 128 from one
+    // to the next, so that eight rows' fragments lie in different banks
+    const int xld = kch * ST_CHUNK * 2 + 16;
+    const int pieces = kch * (ST_CHUNK / 8);  // of 16 bytes, a row
+    for (int r = 0; r < x_rows; r++) {
+        const uint16_t *src = x + (size_t)(SUM ? slot_row[r] : r) * a.ldx;
+        if constexpr (AL16) {
+            for (int i = threadIdx.x; i < pieces; i += ST_T) {  // all in flight together
+                const bool in = i * 8 < a.k;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(xs) + r * xld + i * 16),
+                             "l"(src + (in ? i * 8 : 0)), "r"(in ? 16 : 0)
+                             : "memory");
+            }
+        } else {
+#pragma unroll 4
+            for (int i = threadIdx.x; i < pieces; i += ST_T)
+                *reinterpret_cast<uint4 *>(xs + (size_t)r * xld + i * 16) =
+                    load8<false, false>(src + i * 8, min(a.k - i * 8, 8));
+        }
+    }
+    bool staged = false;  // whether the warp has waited for them
+    auto wait_staged = [&]() {
+        if (staged) return;
+        if (AL16) asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();
+        staged = true;
+    };
+
+    const int total = SUM ? a.n : n_tiles * a.n;
+    const int end = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
+    const int chunks = SUM ? kch * n_tiles : kch;  // steps of one output, split over the warps
+    const int c0 = (int)((long long)chunks * warp / ST_WARPS), c1 = (int)((long long)chunks * (warp + 1) / ST_WARPS);
+    const size_t half = (size_t)a.n * a.ldw;
+    int rb = 0;
+    // groups of up to 16 rows of one expert's features
+    for (int at = (int)((long long)total * blockIdx.x / gridDim.x), rows; at < end; at += rows) {
+        const int out_tile = SUM ? 0 : at / a.n;
+        const int f = at - out_tile * a.n;
+        const int rem = min(end - at, a.n - f), parts = (rem + ST_ROWS - 1) / ST_ROWS;
+        rows = (rem + parts - 1) / parts;
+        const bool row0 = g < rows, row1 = g + 8 < rows;
+        float acc[H][NC][4] = {}, sum[SUM ? NC : 1][4] = {};
+        for (int c = c0; c < c1;) {
+            const int tile = SUM ? c / kch : out_tile;
+            const int first = SUM ? c - tile * kch : c, last = min(kch, first + c1 - c);  // steps of this expert's k
+            c += last - first;
+            const uint16_t *p0 = w + (a.ids ? (size_t)tile_expert[tile] * a.w_expert : 0) + (size_t)(f + g) * a.ldw + 8 * t;
+            const uint16_t *p1 = p0 + 8 * a.ldw;
+            const int used = SUM ? tile_used[tile] : 0;
+            bool in[NC];
+            const uint8_t *xp[NC];
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                const int tok = n * 8 + g;
+                in[n] = SUM ? (used >> tok & 1) != 0 : tok < a.tokens;
+                const int row = SUM ? tile_slot[tile] + __popc(used & ((1 << tok) - 1)) : tok;
+                xp[n] = xs + (size_t)row * xld + 16 * t;
+            }
+            for (int kc = first; kc < last; kc += DEPTH) {
+                uint4 buf[DEPTH][4 * H];
+                if (AL16 && kc + DEPTH <= last && (kc + DEPTH) * ST_CHUNK <= a.k) {
+#pragma unroll
+                    for (int d = 0; d < DEPTH; d++)
+#pragma unroll
+                        for (int h = 0; h < H; h++)
+#pragma unroll
+                            for (int s = 0; s < 2; s++) {
+                                const size_t o = h * half + (size_t)(kc + d) * ST_CHUNK + 32 * s;
+                                buf[d][h * 4 + s] = load8<true, true>(p0 + o, row0 ? 8 : 0);
+                                buf[d][h * 4 + 2 + s] = load8<true, true>(p1 + o, row1 ? 8 : 0);
+                            }
+                } else {
+#pragma unroll
+                    for (int d = 0; d < DEPTH; d++)
+#pragma unroll
+                        for (int h = 0; h < H; h++)
+#pragma unroll
+                            for (int s = 0; s < 2; s++) {
+                                const int k0 = (kc + d) * ST_CHUNK + 32 * s;
+                                const int left = kc + d < last ? min(a.k - k0 - 8 * t, 8) : 0;
+                                const size_t o = h * half + (size_t)k0;
+                                buf[d][h * 4 + s] = load8<AL16, true>(p0 + o, row0 ? left : 0);
+                                buf[d][h * 4 + 2 + s] = load8<AL16, true>(p1 + o, row1 ? left : 0);
+                            }
+                }
+                wait_staged();
+#pragma unroll
+                for (int d = 0; d < DEPTH; d++) {
+                    if (kc + d >= last) break;
+#pragma unroll
+                    for (int n = 0; n < NC; n++)
+#pragma unroll
+                        for (int s = 0; s < 2; s++) {
+                            uint4 xv = make_uint4(0, 0, 0, 0);
+                            if (in[n]) xv = *reinterpret_cast<const uint4 *>(xp[n] + (kc + d) * (ST_CHUNK * 2) + 64 * s);
+#pragma unroll
+                            for (int h = 0; h < H; h++) {
+                                const uint4 lo = buf[d][h * 4 + s], hi = buf[d][h * 4 + 2 + s];
+                                mma16816<T>(acc[h][n], lo.x, hi.x, lo.y, hi.y, xv.x, xv.y);
+                                mma16816<T>(acc[h][n], lo.z, hi.z, lo.w, hi.w, xv.z, xv.w);
+                            }
+                        }
+                }
+            }
+            if constexpr (SUM) {  // the warp's share of this expert's products: weigh it
+#pragma unroll
+                for (int n = 0; n < NC; n++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int tok = n * 8 + 2 * t + (i & 1);
+                        // a token without this expert takes nothing of it, not 0 x inf
+                        if (used >> tok & 1) sum[n][i] = fmaf(tile_w[tile][tok], acc[0][n][i], sum[n][i]);
+                        acc[0][n][i] = 0.0f;
+                    }
+            }
+        }
+        wait_staged();
+#pragma unroll
+        for (int h = 0; h < H; h++)
+#pragma unroll
+            for (int n = 0; n < NC; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    *reinterpret_cast<float2 *>(&red[rb][warp][h][g + 8 * i][n * 8 + 2 * t]) =
+                        SUM ? make_float2(sum[n][2 * i], sum[n][2 * i + 1])
+                            : make_float2(acc[h][n][2 * i], acc[h][n][2 * i + 1]);
+        __syncthreads();
+        // one output a thread: feature f + r of token o
+        const int r = threadIdx.x & 15, o = threadIdx.x >> 4;
+        if (o < COLS && o < a.tokens && r < rows) {
+            float v[1] = {0.0f}, u = 0.0f;
+#pragma unroll
+            for (int i = 0; i < ST_WARPS; i++) {
+                v[0] += red[rb][i][0][r][o];
+                if (GATED) u += red[rb][i][H - 1][r][o];
+            }
+            if (a.bias) v[0] += to_f32(static_cast<const T *>(a.bias)[f + r]);
+            act16(v, a.act);
+            if (GATED) v[0] *= u;
+            if (a.residual) v[0] += to_f32(static_cast<const TY *>(a.residual)[(size_t)o * a.ldr + f + r]);
+            const size_t row = a.ids && !SUM ? (size_t)out_tile * 8 + o : (size_t)o;
+            static_cast<TY *>(a.y)[row * a.ldy + f + r] = from_f32<TY>(v[0]);
+        }
+        rb ^= 1;  // the next group's sums go beside these; the barrier after it frees them
+    }
+}
+
+template <typename T, typename TY, bool GATED, bool SUM, bool AL16, int NC>
+int launch(tpt_cuda_ctx *ctx, const StreamArgs &a, long long rows, int x_rows) {
+    auto kern = k_gemm16_stream<T, TY, GATED, SUM, AL16, NC>;
+    static bool done[64] = {};
+    const int dev = ctx->device & 63;
+    if (!done[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)STREAM_X_BYTES);
+        if (e != cudaSuccess) return cuda_fail(ctx, e, "gemm16_stream smem attribute");
+        done[dev] = true;
+    }
+    const long long grid = rows < 2LL * ctx->sm_count ? rows : 2LL * ctx->sm_count;  // two blocks an SM
+    launch_pdl(kern, (unsigned)grid, ST_T, stream_x_bytes(x_rows, a.k), ctx->stream, a);
+    return after_launch(ctx, "gemm16_stream");
+}
+
+StreamArgs base_args(tpt_cuda_ctx *ctx, const Gemm16 &g) {
+    StreamArgs a = {};
+    a.x = g.x;
+    a.ldx = g.ldx;
+    a.tokens = g.x_rows;
+    a.w = g.w;
+    a.ldw = g.ldw;
+    a.w_expert = g.w_expert;
+    a.n = g.n;
+    a.k = g.k;
+    a.bias = g.bias;
+    a.act = g.act;
+    a.residual = g.residual;
+    a.ldr = g.ldr;
+    a.y = g.y;
+    a.ldy = g.ldy;
+    a.gflags = ctx->d_flags;
+    return a;
+}
+
+template <typename T>
+int dense_typed(tpt_cuda_ctx *ctx, const Gemm16 &g, bool al16) {
+    const StreamArgs a = base_args(ctx, g);
+    auto go = [&](auto ty) {
+        using TY = decltype(ty);
+        if (g.rows <= 8)
+            return al16 ? launch<T, TY, false, false, true, 1>(ctx, a, g.n, g.rows)
+                        : launch<T, TY, false, false, false, 1>(ctx, a, g.n, g.rows);
+        return al16 ? launch<T, TY, false, false, true, 2>(ctx, a, g.n, g.rows)
+                    : launch<T, TY, false, false, false, 2>(ctx, a, g.n, g.rows);
+    };
+    return g.y_f32 ? go(float()) : go(T());
+}
+
+template <typename T>
+int experts_typed(tpt_cuda_ctx *ctx, const Gemm16 &in, const Gemm16 &out, const int *ids, const float *weights,
+                  int pairs, int top_k, bool al16) {
+    StreamArgs a = base_args(ctx, in), b = base_args(ctx, out);
+    a.ids = b.ids = ids;
+    a.weights = b.weights = weights;
+    a.pairs = b.pairs = pairs;
+    a.top_k = b.top_k = top_k;
+    a.experts = b.experts = in.experts;
+    b.tokens = a.tokens;
+    const long long rows = (long long)in.n * (pairs < in.experts ? pairs : in.experts);
+    int st;
+    if (in.gated)
+        st = al16 ? launch<T, T, true, false, true, 1>(ctx, a, rows, a.tokens)
+                  : launch<T, T, true, false, false, 1>(ctx, a, rows, a.tokens);
+    else
+        st = al16 ? launch<T, T, false, false, true, 1>(ctx, a, rows, a.tokens)
+                  : launch<T, T, false, false, false, 1>(ctx, a, rows, a.tokens);
+    if (st) return st;
+    return al16 ? launch<T, T, false, true, true, 1>(ctx, b, out.n, pairs)
+                : launch<T, T, false, true, false, 1>(ctx, b, out.n, pairs);
+}
+
+bool all_aligned(const Gemm16 &g) {
+    return g.k % 8 == 0 && rows16_ok(g.x, g.ldx, (size_t)g.x_rows) && rows16_ok(g.w, g.ldw, 2) &&
+           (g.experts <= 1 || g.w_expert % 8 == 0);
+}
+
+}  // namespace
+
+int launch_gemm16_stream(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
+    const bool al = all_aligned(g);
+    return dtype == TPT_DT_BF16 ? dense_typed<__nv_bfloat16>(ctx, g, al) : dense_typed<__half>(ctx, g, al);
+}
+
+int launch_experts_stream(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &in, const Gemm16 &out, const int *ids,
+                          const float *weights, int pairs, int top_k) {
+    const bool al = all_aligned(in) && all_aligned(out);
+    return dtype == TPT_DT_BF16 ? experts_typed<__nv_bfloat16>(ctx, in, out, ids, weights, pairs, top_k, al)
+                                : experts_typed<__half>(ctx, in, out, ids, weights, pairs, top_k, al);
+}
+
+}  // namespace tpt
