@@ -494,14 +494,14 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
     if (st) return st;
     const void *w_use[2];
     size_t w_ld[2];
+    PadJob job[2];
     for (int i = 0; i < 2; i++) {
         w_use[i] = pad[i] ? (const void *)(ctx->ws + o_w[i]) : (const void *)w_src[i];
         w_ld[i] = pad[i] ? up8(w_k[i]) : w_k[i];
-        if (pad[i]) {
-            st = launch_pad_rows16(ctx, w_src[i], w_k[i], w_rows[i], w_k[i], ctx->ws + o_w[i]);
-            if (st) return st;
-        }
+        if (pad[i]) job[i] = PadJob{w_src[i], w_k[i], w_rows[i], w_k[i], ctx->ws + o_w[i]};
     }
+    st = launch_pad_rows16(ctx, job[0], job[1]);
+    if (st) return st;
     int *pos = (int *)(ctx->ws + o_pos), *tok = gather ? (int *)(ctx->ws + o_tok) : nullptr;
     int *n_tiles = (int *)(ctx->ws + o_n);
     Tile16 *tiles = (Tile16 *)(ctx->ws + o_tiles);

@@ -68,8 +68,14 @@ int launch_experts_stream(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &in, const 
 inline bool rows16_ok(const void *p, size_t ld, size_t rows) {
     return ((uintptr_t)p & 15) == 0 && (rows <= 1 || ld % 8 == 0);
 }
-// dst [rows][k rounded up to a multiple of 8] = src [rows][k], zero-filled
-int launch_pad_rows16(tpt_cuda_ctx *ctx, const void *src, size_t ld, size_t rows, size_t k, void *dst);
+// dst [rows][k rounded up to a multiple of 8, at least 8] = src [rows][k],
+// zero-filled; two of them in one launch
+struct PadJob {
+    const void *src = nullptr;
+    size_t ld = 0, rows = 0, k = 0;
+    void *dst = nullptr;
+};
+int launch_pad_rows16(tpt_cuda_ctx *ctx, const PadJob &a, const PadJob &b);
 
 #ifdef __CUDACC__
 

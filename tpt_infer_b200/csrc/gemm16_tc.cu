@@ -20,6 +20,7 @@
 // Every wait is bounded; a wait that runs out raises the CTA's abort and the
 // context's timeout word, the roles leave, copies and MMAs in flight are
 // drained (bounded), tensor memory is freed and the kernel returns.
+
 #include "gemm16.cuh"
 
 namespace tpt {
@@ -137,72 +138,72 @@ __device__ __forceinline__ void commit_both(uint32_t bar) {
         : "memory");
 }
 
-// The epilogue of C columns (tokens col0 .. col0 + C - 1 of the tile) of this
-// thread's lane. Ungated: lane l of the warp is feature f0 + l, b its bias.
-// Gated: lanes l and l + 16 are the gate and the up product of feature f0 + l;
-// each of them finishes half of the columns. `acc` fills the accumulators; the
-// residual's loads are issued before it. A chunk whose columns are all rows
-// takes the branch-free path, so that its loads and stores go out back to back.
-template <typename TY, bool GATED, int C, typename Acc>
-__device__ __forceinline__ void epilogue16(const Args &a, float b, int f0, size_t row0, int col0, int rows, int lane,
-                                           Acc acc) {
-    float v[C];
-    if constexpr (GATED) {
-        acc(v);
-        const bool hi = lane >= 16;
-        const int f = f0 + (lane & 15);
-        float g[C / 2], u[C / 2];
+// The residual's values of C columns (tokens col0 .. col0 + C - 1 of the tile)
+// of this thread's feature f. A chunk whose columns are all rows takes the
+// branch-free path, here and below, so that its loads and stores go out back to
+// back.
+template <typename TY, int C>
+__device__ __forceinline__ void load_residual(const Args &a, TY (&rv)[C], int f, size_t row0, int col0, int rows) {
+    const int n = f < a.n ? rows - col0 : 0;
+    const TY *r = static_cast<const TY *>(a.residual) + (row0 + col0) * a.ldr + f;
+    if (n >= C) {
 #pragma unroll
-        for (int i = 0; i < C / 2; i++) {
-            const float got = __shfl_xor_sync(0xffffffffu, hi ? v[i] : v[C / 2 + i], 16);
-            g[i] = hi ? got : v[i];
-            u[i] = hi ? v[C / 2 + i] : got;
-        }
-        act16(g, a.act);
-        const int c0 = col0 + (hi ? C / 2 : 0);
-        TY *y = static_cast<TY *>(a.y) + (row0 + c0) * a.ldy + f;
-        const int n = f < a.n ? rows - c0 : 0;
-        if (n >= C / 2) {
-#pragma unroll
-            for (int i = 0; i < C / 2; i++, y += a.ldy) *y = from_f32<TY>(g[i] * u[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < C / 2; i++, y += a.ldy)
-                if (i < n) *y = from_f32<TY>(g[i] * u[i]);
-        }
+        for (int i = 0; i < C; i++, r += a.ldr) rv[i] = *r;
     } else {
-        const int f = f0 + lane;
-        const int n = f < a.n ? rows - col0 : 0;
-        TY rv[C];
-        if (a.residual) {
-            const TY *r = static_cast<const TY *>(a.residual) + (row0 + col0) * a.ldr + f;
-            if (n >= C) {
 #pragma unroll
-                for (int i = 0; i < C; i++, r += a.ldr) rv[i] = *r;
-            } else {
-#pragma unroll
-                for (int i = 0; i < C; i++, r += a.ldr) rv[i] = i < n ? *r : from_f32<TY>(0.0f);
-            }
-        }
-        acc(v);
-#pragma unroll
-        for (int i = 0; i < C; i++) v[i] += b;
-        act16(v, a.act);
-        if (a.residual) {
-#pragma unroll
-            for (int i = 0; i < C; i++) v[i] += to_f32(rv[i]);
-        }
-        TY *y = static_cast<TY *>(a.y) + (row0 + col0) * a.ldy + f;
-        if (n >= C) {
-#pragma unroll
-            for (int i = 0; i < C; i++, y += a.ldy) *y = from_f32<TY>(v[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < C; i++, y += a.ldy)
-                if (i < n) *y = from_f32<TY>(v[i]);
-        }
+        for (int i = 0; i < C; i++, r += a.ldr) rv[i] = i < n ? *r : from_f32<TY>(0.0f);
     }
-    __syncwarp();
+}
+
+// The epilogue of C columns of this thread's lane. Ungated: lane l of the warp
+// is feature f0 + l, b its bias, rv its residual values.
+template <typename TY, int C>
+__device__ __forceinline__ void epilogue16(const Args &a, float (&v)[C], const TY (&rv)[C], float b, int f, size_t row0,
+                                           int col0, int rows) {
+    const int n = f < a.n ? rows - col0 : 0;
+#pragma unroll
+    for (int i = 0; i < C; i++) v[i] += b;
+    act16(v, a.act);
+    if (a.residual) {
+#pragma unroll
+        for (int i = 0; i < C; i++) v[i] += to_f32(rv[i]);
+    }
+    TY *y = static_cast<TY *>(a.y) + (row0 + col0) * a.ldy + f;
+    if (n >= C) {
+#pragma unroll
+        for (int i = 0; i < C; i++, y += a.ldy) *y = from_f32<TY>(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; i++, y += a.ldy)
+            if (i < n) *y = from_f32<TY>(v[i]);
+    }
+}
+// Gated: lanes l and l + 16 are the gate and the up product of feature f0 + l;
+// each of them finishes half of the columns.
+template <typename TY, int C>
+__device__ __forceinline__ void epilogue16_gated(const Args &a, const float (&v)[C], int f0, size_t row0, int col0,
+                                                 int rows, int lane) {
+    const bool hi = lane >= 16;
+    const int f = f0 + (lane & 15);
+    float g[C / 2], u[C / 2];
+#pragma unroll
+    for (int i = 0; i < C / 2; i++) {
+        const float got = __shfl_xor_sync(0xffffffffu, hi ? v[i] : v[C / 2 + i], 16);
+        g[i] = hi ? got : v[i];
+        u[i] = hi ? v[C / 2 + i] : got;
+    }
+    act16(g, a.act);
+    const int c0 = col0 + (hi ? C / 2 : 0);
+    TY *y = static_cast<TY *>(a.y) + (row0 + c0) * a.ldy + f;
+    const int n = f < a.n ? rows - c0 : 0;
+    if (n >= C / 2) {
+#pragma unroll
+        for (int i = 0; i < C / 2; i++, y += a.ldy) *y = from_f32<TY>(g[i] * u[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < C / 2; i++, y += a.ldy)
+            if (i < n) *y = from_f32<TY>(g[i] * u[i]);
+    }
 }
 // the bias of feature f (0: none)
 template <typename T>
@@ -421,18 +422,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             const TileAt tl = tile_at(a, t);
             const int f0 = GATED ? tl.ft * 128 + (int)rank * 64 + q * 16 : tl.ft * 256 + (int)rank * 128 + q * 32;
             const float b = GATED ? 0.0f : bias_at<T>(a, f0 + lane);
+            // the first chunk's residual values and the L2 lines of the others
+            // come while the MMAs run, each further chunk's while the one before
+            // it is finished
+            TY rv[2][32];
+            const bool res = !GATED && a.residual;
+            if (res) {
+                if (half * 32 < tl.rows) load_residual<TY, 32>(a, rv[0], f0 + lane, (size_t)tl.row0, half * 32, tl.rows);
+                for (int c = half * 32 + 64 + lane; c < tl.rows; c += 64)
+                    if (f0 < a.n)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const TY *>(a.residual) +
+                                                                      (size_t)(tl.row0 + c) * a.ldr + f0));
+            }
             int okw = 0;
             if (lane == 0) okw = mbar_wait(tfull_bar(acc), acc_phase, abort_p, a.gflags, true) ? 1 : 0;
             okw = __shfl_sync(0xffffffffu, okw, 0);
             if (!okw) break;
             tc_fence_after();
             const uint32_t t_base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 256);
-#pragma unroll 1
-            for (int c = half * 32; c < tl.rows; c += 64) {
-                epilogue16<TY, GATED, 32>(a, b, f0, (size_t)tl.row0, c, tl.rows, lane, [&](float(&v)[32]) {
-                    tmem_ld32(t_base + (uint32_t)c, reinterpret_cast<uint32_t(&)[32]>(v));
-                    tmem_wait_ld();
-                });
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int c = half * 32 + i * 64;
+                if (c >= tl.rows) break;
+                if (res && c + 64 < tl.rows)
+                    load_residual<TY, 32>(a, rv[(i + 1) & 1], f0 + lane, (size_t)tl.row0, c + 64, tl.rows);
+                float v[32];
+                __syncwarp();
+                tmem_ld32(t_base + (uint32_t)c, reinterpret_cast<uint32_t(&)[32]>(v));
+                tmem_wait_ld();
+                if constexpr (GATED)
+                    epilogue16_gated<TY, 32>(a, v, f0, (size_t)tl.row0, c, tl.rows, lane);
+                else
+                    epilogue16<TY, 32>(a, v, rv[i & 1], b, f0 + lane, (size_t)tl.row0, c, tl.rows);
             }
             tc_fence_before();
             __syncwarp();
@@ -469,7 +490,7 @@ struct SplitCfg {
     static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 3;
     static constexpr int TMEM_COLS = NT < 32 ? 32 : NT;
     static constexpr int SMEM = STAGES * STAGE_BYTES + (2 * STAGES + 1) * 8 + 1024;
-    static_assert(STAGES * STAGE_BYTES >= NT * W_ROWS * 4, "the partial sums reuse the ring");
+
     static_assert(2 * (SMEM + 1024) <= 233472, "two CTAs per SM");
 };
 
@@ -623,21 +644,31 @@ __global__ void __launch_bounds__(S_THREADS, 2)
                 constexpr int C = NT < 32 ? NT : 32;
 #pragma unroll 1
                 for (int c = 0; c < NT && c < rows; c += C) {
-                    epilogue16<TY, GATED, C>(a, b, f0, (size_t)row0, c, rows, lane, [&](float(&v)[C]) {
-                        if constexpr (C == 32)
-                            tmem_ld32(t_base + (uint32_t)c, reinterpret_cast<uint32_t(&)[32]>(v));
-                        else
-                            tmem_ld16(t_base + (uint32_t)c, reinterpret_cast<uint32_t *>(v));
-                        tmem_wait_ld();
-                    });
+                    TY rv[C];
+                    if (!GATED && a.residual) load_residual<TY, C>(a, rv, f0 + lane, (size_t)row0, c, rows);
+                    float v[C];
+                    __syncwarp();
+                    if constexpr (C == 32)
+                        tmem_ld32(t_base + (uint32_t)c, reinterpret_cast<uint32_t(&)[32]>(v));
+                    else
+                        tmem_ld16(t_base + (uint32_t)c, reinterpret_cast<uint32_t *>(v));
+                    tmem_wait_ld();
+                    if constexpr (GATED)
+                        epilogue16_gated<TY, C>(a, v, f0, (size_t)row0, c, rows, lane);
+                    else
+                        epilogue16<TY, C>(a, v, rv, b, f0 + lane, (size_t)row0, c, rows);
                 }
             }
         } else {
-            constexpr int CW = NT / KS;  // columns that each CTA finishes
-            cluster_sync();              // every CTA's MMAs and copies are done: the rings are free
+            // CTA o finishes the columns from o CW on; they lie in its ring as
+            // [source CTA][column][128 features]
+            constexpr int CW = (NT + 4 * KS - 1) / (4 * KS) * 4;
+            constexpr int C = CW % 16 == 0 ? 16 : CW % 8 == 0 ? 8 : 4;
+            static_assert(KS * CW * W_ROWS * 4 <= S * Cfg::STAGE_BYTES, "the partial sums reuse the ring");
+            cluster_sync();  // every CTA's MMAs and copies are done: the rings are free
             if (warp >= 2) {
 #pragma unroll 1
-                for (int c = 0; c < NT; c += 16) {
+                for (int c = 0; c < NT && c < rows; c += 16) {
                     uint32_t v[16];
                     tmem_ld16(t_base + (uint32_t)c, v);
                     tmem_wait_ld();
@@ -652,20 +683,25 @@ __global__ void __launch_bounds__(S_THREADS, 2)
             }
             __syncwarp();
             cluster_sync();
-            const int c0 = rank * CW;
-            if (go && c0 < rows) {
+            const int c0 = rank * CW, c1 = min(min(c0 + CW, NT), rows);
+            if (go) {
                 const float *part = reinterpret_cast<const float *>(smem_raw + (ring - raw)) + q * 32 + lane;
-                constexpr int C = CW < 16 ? CW : 16;
 #pragma unroll 1
-                for (int c = 0; c < CW; c += C) {
-                    epilogue16<TY, GATED, C>(a, b, f0, (size_t)row0, c0 + c, rows, lane, [&](float(&v)[C]) {
+                for (int c = c0; c < c1; c += C) {
+                    TY rv[C];
+                    if (!GATED && a.residual) load_residual<TY, C>(a, rv, f0 + lane, (size_t)row0, c, rows);
+                    float v[C];
 #pragma unroll
-                        for (int i = 0; i < C; i++) {
-                            v[i] = part[(c + i) * W_ROWS];
+                    for (int i = 0; i < C; i++) {
+                        v[i] = part[(c - c0 + i) * W_ROWS];
 #pragma unroll
-                            for (int s = 1; s < KS; s++) v[i] += part[(s * CW + c + i) * W_ROWS];
-                        }
-                    });
+                        for (int s = 1; s < KS; s++) v[i] += part[(s * CW + c - c0 + i) * W_ROWS];
+                    }
+                    if constexpr (GATED)
+                        epilogue16_gated<TY, C>(a, v, f0, (size_t)row0, c, rows, lane);
+                    else
+                        epilogue16<TY, C>(a, v, rv, b, f0 + lane, (size_t)row0, c, rows);
+                    __syncwarp();
                 }
             }
         }
@@ -838,10 +874,14 @@ int launch_split(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
 
 template <typename T, typename TY, bool GATED, int NT>
 int launch_split_k(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g, int ks) {
-    if (ks >= 8) return launch_split<T, TY, GATED, NT, 8>(ctx, dtype, g);
-    if (ks >= 4) return launch_split<T, TY, GATED, NT, 4>(ctx, dtype, g);
-    if (ks >= 2) return launch_split<T, TY, GATED, NT, 2>(ctx, dtype, g);
-    return launch_split<T, TY, GATED, NT, 1>(ctx, dtype, g);
+    switch (ks) {
+        case 8: return launch_split<T, TY, GATED, NT, 8>(ctx, dtype, g);
+        case 6: return launch_split<T, TY, GATED, NT, 6>(ctx, dtype, g);
+        case 4: return launch_split<T, TY, GATED, NT, 4>(ctx, dtype, g);
+        case 3: return launch_split<T, TY, GATED, NT, 3>(ctx, dtype, g);
+        case 2: return launch_split<T, TY, GATED, NT, 2>(ctx, dtype, g);
+        default: return launch_split<T, TY, GATED, NT, 1>(ctx, dtype, g);
+    }
 }
 
 template <typename T, typename TY, bool GATED>
@@ -852,8 +892,13 @@ int launch_tc(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
     if (g.tiles ? g.tile_rows > 128 : g.rows > 256) return launch_pair<T, TY, GATED>(ctx, dtype, g, 256);
     const int nt = g.tiles ? g.tile_rows : g.rows <= 16 ? 16 : g.rows <= 32 ? 32 : g.rows <= 64 ? 64 : 128;
     const long long tiles = (g.tiles ? (long long)g.max_tiles : ((long long)g.rows + nt - 1) / nt) * ft;
+    // How many CTAs share a tile's k: as many as are resident at once, three steps
+    // each at least. Measured at 32 tiles of 4096 values: 1 25 us, 2 15, 4 and up
+    // 10.3; at 86 tiles: 1 27.6, 2 21.9, 3 20.9, 4 27.1 (a third round). The wide
+    // tile's exchange costs more than its eighth share saves.
     int ks = 1;
-    while (ks < 8 && tiles * ks * 2 <= 2LL * ctx->sm_count && kb / (ks * 2) >= 4) ks *= 2;
+    for (int s : {2, 3, 4, 6, 8})
+        if (tiles * s <= 2LL * ctx->sm_count && kb / s >= 3 && (nt < 128 || s <= 4)) ks = s;
     if (nt == 16) return launch_split_k<T, TY, GATED, 16>(ctx, dtype, g, ks);
     if (nt == 32) return launch_split_k<T, TY, GATED, 32>(ctx, dtype, g, ks);
     if (nt == 64) return launch_split_k<T, TY, GATED, 64>(ctx, dtype, g, ks);
