@@ -111,6 +111,21 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap *tm,
         : "memory");
 }
 
+// The producer and the MMA issuer run as whole warps with uniform control flow
+// and elect one lane for the issue itself: descriptors, addresses and
+// coordinates then stay in uniform registers. (One diverged lane doing it all
+// moved each of them over again: 75 cycles an MMA, 600 a stage, twice the
+// tensor cores' own time.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, unsigned *gflags,
+                                          bool honour_abort) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, gflags, honour_abort));
+}
+
 template <int GROUP>
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -281,7 +296,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     auto tempty_bar = [&](int b) { return bars + 8u * (2 * S + 2 + b); };
     const uint32_t drain_bar = bars + 8u * (2 * S + 4);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const bool leader = rank == 0;
     const int cluster = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
@@ -318,8 +333,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     const int ntiles = a.tiles ? __ldcg(a.n_tiles) * a.ftiles : ((a.rows + a.tile_n - 1) / a.tile_n) * a.ftiles;
 
     if (warp == 0) {
-        if (lane == 0) {
         // ---------------- producer ----------------
+        const uint32_t full_leader = map_to_rank(full_bar(0), 0);
         int stage = 0;
         uint32_t phase = 0;
         int issued = 0;
@@ -330,25 +345,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             const int box = half > 64 ? 0 : half > 32 ? 1 : 2;
             const uint32_t bytes = 2u * (W_BYTES + (W_BYTES >> box));
             const int xrow = tl.row0 + (int)rank * half;
+            const CUtensorMap *xmap = &tmX.box[box];
             for (int kb = 0; kb < kblocks; kb++) {
-                if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_p, a.gflags, true)) {
+                if (!warp_wait(empty_bar(stage), phase ^ 1u, abort_p, a.gflags, true)) {
                     ok = false;
                     break;
                 }
                 const uint32_t w_dst = ring + stage * P_STAGE_BYTES, x_dst = w_dst + W_BYTES;
-                const uint32_t fb = map_to_rank(full_bar(stage), 0);
-                if (leader) mbar_arrive_expect_tx(full_bar(stage), bytes);
-                if (GATED && a.gate16) {
-                    tma_load_5d_p(w_dst, &tmW, fb, kb * BK, 0, 0, tl.ft * 8 + (int)rank * 4, tl.expert);
-                } else if (GATED) {
+                const uint32_t fb = full_leader + 8u * stage;
+                if (elect_one()) {
+                    if (leader) mbar_arrive_expect_tx(full_bar(stage), bytes);
+                    if (GATED && a.gate16) {
+                        tma_load_5d_p(w_dst, &tmW, fb, kb * BK, 0, 0, tl.ft * 8 + (int)rank * 4, tl.expert);
+                    } else if (GATED) {
 #pragma unroll
-                    for (int q = 0; q < 4; q++)
-                        tma_load_4d_p(w_dst + q * 4096, &tmW, fb, kb * BK, tl.ft * 128 + (int)rank * 64 + q * 16, 0,
-                                      tl.expert);
-                } else {
-                    tma_load_3d_p(w_dst, &tmW, fb, kb * BK, tl.ft * 256 + (int)rank * 128, tl.expert);
+                        for (int q = 0; q < 4; q++)
+                            tma_load_4d_p(w_dst + q * 4096, &tmW, fb, kb * BK, tl.ft * 128 + (int)rank * 64 + q * 16,
+                                          0, tl.expert);
+                    } else {
+                        tma_load_3d_p(w_dst, &tmW, fb, kb * BK, tl.ft * 256 + (int)rank * 128, tl.expert);
+                    }
+                    tma_load_2d_p(x_dst, xmap, fb, kb * BK, xrow);
                 }
-                tma_load_2d_p(x_dst, &tmX.box[box], fb, kb * BK, xrow);
+                __syncwarp();
                 issued++;
                 if (++stage == S) {
                     stage = 0;
@@ -365,12 +384,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     stage = S - 1;
                     phase ^= 1u;
                 }
-                mbar_wait(full_bar(stage), phase, abort_p, a.gflags, false);
+                warp_wait(full_bar(stage), phase, abort_p, a.gflags, false);
             }
         }
-        }
     } else if (warp == 1) {
-        if (lane == 0 && leader) {
+        if (leader) {
             // ---------------- MMA issuer ----------------
             int stage = 0;
             uint32_t phase = 0;
@@ -379,37 +397,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             bool ok = true;
             for (int t = cluster; t < ntiles && ok; t += nclusters) {
                 const uint32_t idesc = idesc_f16(a.fmt, 256, tile_at(a, t).cols);
-                if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_p, a.gflags, true)) break;
+                if (!warp_wait(tempty_bar(acc), acc_phase ^ 1u, abort_p, a.gflags, true)) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem + (uint32_t)(acc * 256);
                 for (int kb = 0; kb < kblocks; kb++) {
-                    if (!mbar_wait(full_bar(stage), phase, abort_p, a.gflags, true)) {
+                    if (!warp_wait(full_bar(stage), phase, abort_p, a.gflags, true)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint32_t w_addr = ring + stage * P_STAGE_BYTES, x_addr = w_addr + W_BYTES;
+                    const uint64_t wd = sw128_desc(w_addr), xd = sw128_desc(x_addr);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < BK / 16; kk++)
-                        mma_f16<2>(d_tmem, sw128_desc(w_addr + 32 * kk), sw128_desc(x_addr + 32 * kk), idesc,
-                                   (kb | kk) != 0 ? 1u : 0u);
-                    commit_both(empty_bar(stage));
+                        for (int kk = 0; kk < BK / 16; kk++)
+                            mma_f16<2>(d_tmem, wd + 2 * kk, xd + 2 * kk, idesc, (kb | kk) != 0 ? 1u : 0u);
+                        commit_both(empty_bar(stage));
+                    }
+                    __syncwarp();
                     if (++stage == S) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
                 if (!ok) break;
-                commit_both(tfull_bar(acc));
+                if (elect_one()) commit_both(tfull_bar(acc));
+                __syncwarp();
                 if (++acc == 2) {
                     acc = 0;
                     acc_phase ^= 1u;
                 }
             }
             // drain: every MMA issued completes before tensor memory is freed
-            asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain_bar)
-                         : "memory");
-            mbar_wait(drain_bar, 0, abort_p, a.gflags, false);
+            if (elect_one())
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                                 drain_bar)
+                             : "memory");
+            __syncwarp();
+            warp_wait(drain_bar, 0, abort_p, a.gflags, false);
         }
     } else {
         // ---------------- epilogue: two warps per lane quarter, alternate 32-column chunks ----------------
@@ -509,7 +534,7 @@ __global__ void __launch_bounds__(S_THREADS, 2)
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
     const uint32_t done_bar = bars + 8u * (2 * S);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = KS > 1 ? (int)cluster_rank() : 0;
 
     if (threadIdx.x == 0) {
@@ -567,12 +592,11 @@ __global__ void __launch_bounds__(S_THREADS, 2)
             int stage = 0, issued = 0;
             uint32_t phase = 0;
             for (int kb = kb0; kb < kb1; kb++) {
-                if (lane == 0) ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_p, a.gflags, true);
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+                ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_p, a.gflags, true);
                 if (!ok) break;
                 const uint32_t w_dst = ring + stage * Cfg::STAGE_BYTES, x_dst = w_dst + W_BYTES;
                 const uint32_t fb = full_bar(stage);
-                if (lane == 0) {
+                if (elect_one()) {
                     mbar_arrive_expect_tx(fb, Cfg::STAGE_BYTES);
                     if (GATED && a.gate16) {
                         tma_load_5d(w_dst, &tmW, fb, kb * BK, 0, 0, ft * 4, expert);
@@ -593,39 +617,41 @@ __global__ void __launch_bounds__(S_THREADS, 2)
                     phase ^= 1u;
                 }
             }
-            if (!ok && lane == 0) {  // aborting: no copy stays in flight
+            if (!ok) {  // aborting: no copy stays in flight
                 const int n = issued < S ? issued : S;
                 for (int i = 0; i < n; i++) {
                     if (--stage < 0) {
                         stage = S - 1;
                         phase ^= 1u;
                     }
-                    mbar_wait(full_bar(stage), phase, abort_p, a.gflags, false);
+                    warp_wait(full_bar(stage), phase, abort_p, a.gflags, false);
                 }
             }
         } else if (warp == 1) {
-            if (lane == 0) {
-                // ---------------- MMA issuer ----------------
-                const uint32_t idesc = idesc_f16(a.fmt, 128, NT);
-                int stage = 0;
-                uint32_t phase = 0;
-                for (int kb = kb0; kb < kb1; kb++) {
-                    if (!mbar_wait(full_bar(stage), phase, abort_p, a.gflags, true)) break;
-                    tc_fence_after();
-                    const uint32_t w_addr = ring + stage * Cfg::STAGE_BYTES, x_addr = w_addr + W_BYTES;
+            // ---------------- MMA issuer ----------------
+            const uint32_t idesc = idesc_f16(a.fmt, 128, NT);
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (!warp_wait(full_bar(stage), phase, abort_p, a.gflags, true)) break;
+                tc_fence_after();
+                const uint32_t w_addr = ring + stage * Cfg::STAGE_BYTES, x_addr = w_addr + W_BYTES;
+                const uint64_t wd = sw128_desc(w_addr), xd = sw128_desc(x_addr);
+                if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; kk++)
-                        mma_f16<1>(tmem, sw128_desc(w_addr + 32 * kk), sw128_desc(x_addr + 32 * kk), idesc,
-                                   kb > kb0 || kk > 0 ? 1u : 0u);
+                        mma_f16<1>(tmem, wd + 2 * kk, xd + 2 * kk, idesc, kb > kb0 || kk > 0 ? 1u : 0u);
                     tc_commit(empty_bar(stage));
-                    if (++stage == S) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
                 }
-                tc_commit(done_bar);
-                mbar_wait(done_bar, 0, abort_p, a.gflags, false);
+                __syncwarp();
+                if (++stage == S) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
             }
+            if (elect_one()) tc_commit(done_bar);
+            __syncwarp();
+            warp_wait(done_bar, 0, abort_p, a.gflags, false);
         }
         // ---------------- epilogue (warps 2 to 5) ----------------
         const int q = warp & 3;
