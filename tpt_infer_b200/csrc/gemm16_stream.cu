@@ -84,12 +84,12 @@ __device__ __forceinline__ uint4 load8(const uint16_t *p, int n) {
 
 // GATED: y = act(W x) * (W2 x). SUM: y[token] = sum over the experts of
 // weight * W_e x_e, x the tiles' rows [tile][token]; otherwise each tile's
-// products go to y's rows [tile][token] (dense: one tile). NC: tokens / 8.
-template <typename T, typename TY, bool GATED, bool SUM, bool AL16, int NC>
+// products go to y's rows [tile][token] (dense: one tile). Up to 8 tokens.
+template <typename T, typename TY, bool GATED, bool SUM, bool AL16>
 __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant__ StreamArgs a) {
     constexpr int H = GATED ? 2 : 1;
     constexpr int DEPTH = GATED ? 2 : 4;  // steps in flight: 16 loads of 16 bytes a thread
-    constexpr int COLS = 8 * NC;
+    constexpr int COLS = 8;
     __shared__ float red[2][ST_WARPS][H][ST_ROWS][COLS];
     __shared__ int tile_expert[32];
     __shared__ float tile_w[SUM ? 32 : 1][8];
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
         const int rem = min(end - at, a.n - f), parts = (rem + ST_ROWS - 1) / ST_ROWS;
         rows = (rem + parts - 1) / parts;
         const bool row0 = g < rows, row1 = g + 8 < rows;
-        float acc[H][NC][4] = {}, sum[SUM ? NC : 1][4] = {};
+        float acc[H][4] = {}, sum[4] = {};
         for (int c = c0; c < c1;) {
             const int tile = SUM ? c / kch : out_tile;
             const int first = SUM ? c - tile * kch : c, last = min(kch, first + c1 - c);  // steps of this expert's k
@@ -197,15 +197,9 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
             const uint16_t *p0 = w + (a.ids ? (size_t)tile_expert[tile] * a.w_expert : 0) + (size_t)(f + g) * a.ldw + 8 * t;
             const uint16_t *p1 = p0 + 8 * a.ldw;
             const int used = SUM ? tile_used[tile] : 0;
-            bool in[NC];
-            const uint8_t *xp[NC];
-#pragma unroll
-            for (int n = 0; n < NC; n++) {
-                const int tok = n * 8 + g;
-                in[n] = SUM ? (used >> tok & 1) != 0 : tok < a.tokens;
-                const int row = SUM ? tile_slot[tile] + __popc(used & ((1 << tok) - 1)) : tok;
-                xp[n] = xs + (size_t)row * xld + 16 * t;
-            }
+            // this lane's column is token g
+            const bool in = SUM ? (used >> g & 1) != 0 : g < a.tokens;
+            const uint8_t *xp = xs + (size_t)(SUM ? tile_slot[tile] + __popc(used & ((1 << g) - 1)) : g) * xld + 16 * t;
             for (int kc = first; kc < last; kc += DEPTH) {
                 uint4 buf[DEPTH][4 * H];
                 if (AL16 && kc + DEPTH <= last && (kc + DEPTH) * ST_CHUNK <= a.k) {
@@ -238,42 +232,34 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
                 for (int d = 0; d < DEPTH; d++) {
                     if (kc + d >= last) break;
 #pragma unroll
-                    for (int n = 0; n < NC; n++)
+                    for (int s = 0; s < 2; s++) {
+                        uint4 xv = make_uint4(0, 0, 0, 0);
+                        if (in) xv = *reinterpret_cast<const uint4 *>(xp + (kc + d) * (ST_CHUNK * 2) + 64 * s);
 #pragma unroll
-                        for (int s = 0; s < 2; s++) {
-                            uint4 xv = make_uint4(0, 0, 0, 0);
-                            if (in[n]) xv = *reinterpret_cast<const uint4 *>(xp[n] + (kc + d) * (ST_CHUNK * 2) + 64 * s);
-#pragma unroll
-                            for (int h = 0; h < H; h++) {
-                                const uint4 lo = buf[d][h * 4 + s], hi = buf[d][h * 4 + 2 + s];
-                                mma16816<T>(acc[h][n], lo.x, hi.x, lo.y, hi.y, xv.x, xv.y);
-                                mma16816<T>(acc[h][n], lo.z, hi.z, lo.w, hi.w, xv.z, xv.w);
-                            }
+                        for (int h = 0; h < H; h++) {
+                            const uint4 lo = buf[d][h * 4 + s], hi = buf[d][h * 4 + 2 + s];
+                            mma16816<T>(acc[h], lo.x, hi.x, lo.y, hi.y, xv.x, xv.y);
+                            mma16816<T>(acc[h], lo.z, hi.z, lo.w, hi.w, xv.z, xv.w);
                         }
+                    }
                 }
             }
             if constexpr (SUM) {  // the warp's share of this expert's products: weigh it
 #pragma unroll
-                for (int n = 0; n < NC; n++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int tok = n * 8 + 2 * t + (i & 1);
-                        // a token without this expert takes nothing of it, not 0 x inf
-                        if (used >> tok & 1) sum[n][i] = fmaf(tile_w[tile][tok], acc[0][n][i], sum[n][i]);
-                        acc[0][n][i] = 0.0f;
-                    }
+                for (int i = 0; i < 4; i++) {
+                    const int tok = 2 * t + (i & 1);
+                    // a token without this expert takes nothing of it, not 0 x inf
+                    if (used >> tok & 1) sum[i] = fmaf(tile_w[tile][tok], acc[0][i], sum[i]);
+                    acc[0][i] = 0.0f;
+                }
             }
         }
         wait_staged();
 #pragma unroll
         for (int h = 0; h < H; h++)
-#pragma unroll
-            for (int n = 0; n < NC; n++)
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-                    *reinterpret_cast<float2 *>(&red[rb][warp][h][g + 8 * i][n * 8 + 2 * t]) =
-                        SUM ? make_float2(sum[n][2 * i], sum[n][2 * i + 1])
-                            : make_float2(acc[h][n][2 * i], acc[h][n][2 * i + 1]);
+            for (int i = 0; i < 2; i++)
+                *reinterpret_cast<float2 *>(&red[rb][warp][h][g + 8 * i][2 * t]) =
+                    SUM ? make_float2(sum[2 * i], sum[2 * i + 1]) : make_float2(acc[h][2 * i], acc[h][2 * i + 1]);
         __syncthreads();
         // one output a thread: feature f + r of token o
         const int r = threadIdx.x & 15, o = threadIdx.x >> 4;
@@ -295,9 +281,9 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
     }
 }
 
-template <typename T, typename TY, bool GATED, bool SUM, bool AL16, int NC>
+template <typename T, typename TY, bool GATED, bool SUM, bool AL16>
 int launch(tpt_cuda_ctx *ctx, const StreamArgs &a, long long rows, int x_rows) {
-    auto kern = k_gemm16_stream<T, TY, GATED, SUM, AL16, NC>;
+    auto kern = k_gemm16_stream<T, TY, GATED, SUM, AL16>;
     static bool done[64] = {};
     const int dev = ctx->device & 63;
     if (!done[dev]) {
@@ -335,11 +321,8 @@ int dense_typed(tpt_cuda_ctx *ctx, const Gemm16 &g, bool al16) {
     const StreamArgs a = base_args(ctx, g);
     auto go = [&](auto ty) {
         using TY = decltype(ty);
-        if (g.rows <= 8)
-            return al16 ? launch<T, TY, false, false, true, 1>(ctx, a, g.n, g.rows)
-                        : launch<T, TY, false, false, false, 1>(ctx, a, g.n, g.rows);
-        return al16 ? launch<T, TY, false, false, true, 2>(ctx, a, g.n, g.rows)
-                    : launch<T, TY, false, false, false, 2>(ctx, a, g.n, g.rows);
+        return al16 ? launch<T, TY, false, false, true>(ctx, a, g.n, g.rows)
+                    : launch<T, TY, false, false, false>(ctx, a, g.n, g.rows);
     };
     return g.y_f32 ? go(float()) : go(T());
 }
@@ -357,14 +340,14 @@ int experts_typed(tpt_cuda_ctx *ctx, const Gemm16 &in, const Gemm16 &out, const 
     const long long rows = (long long)in.n * (pairs < in.experts ? pairs : in.experts);
     int st;
     if (in.gated)
-        st = al16 ? launch<T, T, true, false, true, 1>(ctx, a, rows, a.tokens)
-                  : launch<T, T, true, false, false, 1>(ctx, a, rows, a.tokens);
+        st = al16 ? launch<T, T, true, false, true>(ctx, a, rows, a.tokens)
+                  : launch<T, T, true, false, false>(ctx, a, rows, a.tokens);
     else
-        st = al16 ? launch<T, T, false, false, true, 1>(ctx, a, rows, a.tokens)
-                  : launch<T, T, false, false, false, 1>(ctx, a, rows, a.tokens);
+        st = al16 ? launch<T, T, false, false, true>(ctx, a, rows, a.tokens)
+                  : launch<T, T, false, false, false>(ctx, a, rows, a.tokens);
     if (st) return st;
-    return al16 ? launch<T, T, false, true, true, 1>(ctx, b, out.n, pairs)
-                : launch<T, T, false, true, false, 1>(ctx, b, out.n, pairs);
+    return al16 ? launch<T, T, false, true, true>(ctx, b, out.n, pairs)
+                : launch<T, T, false, true, false>(ctx, b, out.n, pairs);
 }
 
 bool all_aligned(const Gemm16 &g) {

@@ -859,6 +859,32 @@ int launch_pair(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g, int tile_n) {
     return after_launch(ctx, "gemm16_pair");
 }
 
+// Tokens per tile of a dense product: the fewest cycles by a model of the pair
+// kernel. A stage of 64 k values takes ~240 + 1.1 N cycles (521 at N = 256,
+// where the MMAs alone take 512), a tile's epilogue ~20 N (more with a residual
+// or a smooth activation) and runs beside the next tile's stages; what counts
+// are the rounds of tiles over the pairs and the last tile's epilogue.
+// Measured: 8192 x 768 x 768 with residual 18.4 us at 256, 15.3 at 176, 14.9 at
+// 128, 18.9 at 64; 512 x 4096 x 4096 25.1 at 256, 19.3 at 128; 4096^3 97 at 256,
+// 119 at 128.
+int pair_tile_n(tpt_cuda_ctx *ctx, const Gemm16 &g) {
+    const long long pairs = ctx->sm_count / 2 > 0 ? ctx->sm_count / 2 : 1;
+    const long long ft = (g.n + 255) / 256, kb = (g.k + BK - 1) / BK;
+    int best_n = 256;
+    double best = 0.0;
+    for (int n : {256, 224, 192, 176, 160, 128, 96, 64, 32}) {
+        const long long tiles = ((g.rows + n - 1) / n) * ft, rounds = (tiles + pairs - 1) / pairs;
+        const double main = (double)kb * (240 + 1.1 * n);
+        const double epi = n * (20.0 + (g.residual ? 5 : 0) + (g.act == TPT_ACT_GELU || g.act == TPT_ACT_SILU ? 12 : 0));
+        const double t = main + (double)(rounds - 1) * (main > epi ? main : epi) + epi;
+        if (n == 256 || t < best) {
+            best = t;
+            best_n = n;
+        }
+    }
+    return best_n;
+}
+
 template <typename T, typename TY, bool GATED, int NT, int KS>
 int launch_split(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
     using Cfg = SplitCfg<NT>;
@@ -915,7 +941,13 @@ int launch_tc(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
     const int fw = GATED ? 64 : 128;  // features of a split tile
     const long long ft = (g.n + fw - 1) / fw;
     const int kb = (g.k + BK - 1) / BK;
-    if (g.tiles ? g.tile_rows > 128 : g.rows > 256) return launch_pair<T, TY, GATED>(ctx, dtype, g, 256);
+    // More than 128 tokens go to the pair kernel; 65 to 128 do where its tiles
+    // reach half of the pairs or k is too short to be worth splitting (80 x 1024 x
+    // 11008: 8.7 us against 11.4, 128 x 768 x 768: 5.3 against 6.1; but 128 x 4096
+    // x 4096: 16.9 against 13.9).
+    const bool pair = g.tiles ? g.tile_rows > 128
+                              : g.rows > 128 || (g.rows > 64 && (((g.n + 255LL) / 256) * 4 >= ctx->sm_count || kb <= 16));
+    if (pair) return launch_pair<T, TY, GATED>(ctx, dtype, g, g.tiles ? 256 : pair_tile_n(ctx, g));
     const int nt = g.tiles ? g.tile_rows : g.rows <= 16 ? 16 : g.rows <= 32 ? 32 : g.rows <= 64 ? 64 : 128;
     const long long tiles = (g.tiles ? (long long)g.max_tiles : ((long long)g.rows + nt - 1) / nt) * ft;
     // How many CTAs share a tile's k: as many as are resident at once, three steps
