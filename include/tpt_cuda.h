@@ -436,7 +436,8 @@ int tpt_cuda_linear_dev(tpt_cuda_ctx *ctx, int dtype, const void *x, size_t ldx,
  * the groups_kept best groups (ties: lowest index) stay. The top_k best
  * experts' indices go to ids [tokens, top_k], best first, their s (without the
  * bias) to weights, divided by their sum if renormalise, times scale.
- * A logit of -inf or NaN (or such a bias) takes its expert out; where fewer
+ * A sigmoid logit under -87 scores 0. A logit of -inf or NaN (or such a
+ * bias) takes its expert out; where fewer
  * than top_k experts are left, the rest of ids is -1 with weight 0, and so is
  * every entry of a token whose mask byte is 0 (mask [tokens] or NULL).
  * top_k must not exceed the experts of groups_kept groups. */

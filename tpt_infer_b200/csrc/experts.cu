@@ -55,11 +55,16 @@ __device__ __forceinline__ void load_logits(const T *p, bool vec, int n, float (
         for (int i = 0; i < V; i++) s[i] = i < n ? to_f32(p[i]) : -INFINITY;
     }
 }
-// the score of one logit: the largest logit itself by comparison, so that its
-// term is 1 for +inf too
-__device__ __forceinline__ float route_score(float l, bool softmax, float top, float rsum) {
-    if (l == -INFINITY) return 0.0f;
-    return softmax ? (l == top ? 1.0f : expf(l - top)) * rsum : __frcp_rn(1.0f + expf(-l));
+// A logit's share of the softmax before the division by the sum; the largest
+// logit itself by comparison, so that its term is 1 for +inf too.
+__device__ __forceinline__ float softmax_term(float l, float top) { return l == top ? 1.0f : expf(l - top); }
+// 1 / (1 + e^-l): the hardware's reciprocal and one Newton step. Under -87 (a
+// score below 2^-125) it is 0, since e^-l may not be finite there.
+__device__ __forceinline__ float sigmoid_score(float l) {
+    const float d = 1.0f + expf(-fmaxf(l, -87.0f));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    return l < -87.0f ? 0.0f : fmaf(r, fmaf(-d, r, 1.0f), r);
 }
 
 // One warp per token. Each group has `lanes` (a power of two) neighbouring
@@ -90,87 +95,95 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32)
         float c[V];
         load_logits<T, V>(row + e0, vec, n, c);
         float top = NEG, rsum = 1.0f;
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            c[i] = c[i] > NEG ? c[i] : NEG;  // NaN: an expert that cannot be chosen
-            top = fmaxf(top, c[i]);
-        }
         if (softmax) {
+#pragma unroll
+            for (int i = 0; i < V; i++) top = fmaxf(top, c[i]);  // NaN: the other operand
             top = warp_max(top);
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const float s = route_score(c[i], true, top, 1.0f);
+                const float s = c[i] > NEG ? softmax_term(c[i], top) : 0.0f;
                 sum += s;
-                c[i] = c[i] == NEG ? NEG : s;
+                c[i] = c[i] > NEG ? s : NEG;  // NaN and -inf: experts that cannot be chosen
             }
             sum = warp_sum(sum);
             rsum = sum > 0.0f ? __frcp_rn(sum) : 0.0f;
 #pragma unroll
-            for (int i = 0; i < V; i++) c[i] = c[i] == NEG ? NEG : c[i] * rsum;
+            for (int i = 0; i < V; i++) c[i] = c[i] > NEG ? c[i] * rsum : NEG;
         } else {
 #pragma unroll
-            for (int i = 0; i < V; i++) c[i] = c[i] == NEG ? NEG : route_score(c[i], false, 0.0f, 1.0f);
+            for (int i = 0; i < V; i++) c[i] = c[i] > NEG ? sigmoid_score(c[i]) : NEG;
         }
         if (bias) {
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const float b = c[i] == NEG ? NEG : c[i] + (i < n ? __ldg(bias + e0 + i) : 0.0f);
-                c[i] = b > NEG ? b : NEG;  // a NaN or -inf bias switches the expert off
+                const float b = c[i] + (i < n ? __ldg(bias + e0 + i) : 0.0f);
+                c[i] = c[i] > NEG && b > NEG ? b : NEG;  // a NaN or -inf bias switches the expert off
             }
         }
-        if (groups > 1) {
-            float b1 = NEG, b2 = NEG;
+        // This lane's best two, the lower index first among equals; `gone` marks
+        // the ones already chosen.
+        float b1, b2;
+        int i1, i2;
+        unsigned long long gone = 0;
+        auto scan = [&]() {
+            b1 = b2 = NEG;
+            i1 = i2 = 0;
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                b2 = fmaxf(b2, fminf(b1, c[i]));
-                b1 = fmaxf(b1, c[i]);
+                const float v = gone >> i & 1 ? NEG : c[i];
+                const bool first = v > b1, second = v > b2;
+                i2 = first ? i1 : second ? i : i2;
+                b2 = fmaxf(b2, fminf(b1, v));
+                i1 = first ? i : i1;
+                b1 = fmaxf(b1, v);
             }
+        };
+        scan();
+        if (groups > 1) {
+            float g1 = b1, g2 = b2;
             for (int o = 1; o < lanes; o <<= 1) {
-                const float p1 = __shfl_xor_sync(0xffffffffu, b1, o), p2 = __shfl_xor_sync(0xffffffffu, b2, o);
-                b2 = fmaxf(fminf(b1, p1), fmaxf(b2, p2));
-                b1 = fmaxf(b1, p1);
+                const float p1 = __shfl_xor_sync(0xffffffffu, g1, o), p2 = __shfl_xor_sync(0xffffffffu, g2, o);
+                g2 = fmaxf(fminf(g1, p1), fmaxf(g2, p2));
+                g1 = fmaxf(g1, p1);
             }
-            const float mine = group_top == 2 && b2 > NEG ? b1 + b2 : b1;
+            const float mine = group_top == 2 && g2 > NEG ? g1 + g2 : g1;
             int better = 0;
             for (int g = 0; g < groups; g++) {
                 const float o = __shfl_sync(0xffffffffu, mine, g * lanes);
                 better += o > mine || (o == mine && g < q) ? 1 : 0;
             }
-            if (better >= groups_kept) {
-#pragma unroll
-                for (int i = 0; i < V; i++) c[i] = NEG;
+            if (better >= groups_kept) {  // nothing of this lane can be chosen
+                b1 = b2 = NEG;
+                gone = ~0ull;
             }
         }
-        float b = NEG;
-        int at = 0;
-#pragma unroll
-        for (int i = 0; i < V; i++)
-            if (c[i] > b) {
-                b = c[i];
-                at = i;
-            }
+        int cached = 2;  // how many of (b1, b2) stand
         for (int j = 0; j < top_k; j++) {
-            const unsigned key = order_key(b + 0.0f);  // -0 counts as 0
+            const unsigned key = order_key(b1 + 0.0f);  // -0 counts as 0
             const unsigned best = __reduce_max_sync(0xffffffffu, key);
             if (best == order_key(NEG)) break;  // no expert is left
             const int owner = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1;
-            const int e = __shfl_sync(0xffffffffu, e0 + at, owner);
+            const int e = __shfl_sync(0xffffffffu, e0 + i1, owner);
             if (lane == j) id_mine = e;
             if (lane == owner) {
-                const int gone = at;
-                b = NEG;
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    if (i == gone) c[i] = NEG;
-                    if (c[i] > b) {
-                        b = c[i];
-                        at = i;
-                    }
+                gone |= 1ull << i1;
+                b1 = b2;
+                i1 = i2;
+                cached--;
+            }
+            if (V > 1 && __any_sync(0xffffffffu, cached == 0)) {
+                if (cached == 0) {
+                    scan();
+                    cached = 2;
                 }
             }
+            if (V == 1 && lane == owner) b1 = NEG;
         }
-        if (id_mine >= 0) w_mine = route_score(to_f32(row[id_mine]), softmax, top, rsum);
+        if (id_mine >= 0) {
+            const float l = to_f32(row[id_mine]);
+            w_mine = softmax ? softmax_term(l, top) * rsum : sigmoid_score(l);
+        }
         if (renormalise) {
             const float sum = warp_sum(w_mine);
             w_mine = sum > 0.0f ? w_mine / sum : 0.0f;
@@ -423,62 +436,33 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
                 bool gated, const T *residual, size_t ldr, T *y, size_t ldy) {
     auto up8 = [](size_t v) { return (v + 7) / 8 * 8; };
     const size_t ldh = up8(f), lds = up8(d), ldp = (d + 3) / 4 * 4;  // rows start on 16 bytes
-    if (tokens <= 8 && tokens * top_k <= STREAM_PAIRS && stream_x_bytes(tokens, d) <= STREAM_X_BYTES &&
-        stream_x_bytes(tokens * top_k, f) <= STREAM_X_BYTES) {
-        const size_t tiles = tokens * top_k < experts ? tokens * top_k : experts;
-        int st = ensure_ws(ctx, tiles * 8 * ldh * 2);
-        if (st) return st;
-        Gemm16 g;
-        g.x = x;
-        g.ldx = ldx;
-        g.x_rows = (int)tokens;
-        g.w = w_in;
-        g.ldw = d;
-        g.w_expert = (gated ? 2 : 1) * f * d;
-        g.n = (int)f;
-        g.k = (int)d;
-        g.experts = (int)experts;
-        g.act = act;
-        g.gated = gated;
-        g.y = ctx->ws;
-        g.ldy = ldh;
-        Gemm16 o;
-        o.x = ctx->ws;
-        o.ldx = ldh;
-        o.x_rows = 8;
-        o.w = w_out;
-        o.ldw = f;
-        o.w_expert = d * f;
-        o.n = (int)d;
-        o.k = (int)f;
-        o.experts = (int)experts;
-        o.residual = residual;
-        o.ldr = ldr;
-        o.y = y;
-        o.ldy = ldy;
-        return launch_experts_stream(ctx, dtype, g, o, ids, weights, (int)(tokens * top_k), (int)top_k);
-    }
+    const bool x_ok = d % 8 == 0 && rows16_ok(x, ldx, tokens);
     // Tokens per tile of the products: what an expert gets on average, up to the
     // pair kernel's 256 columns.
     const size_t mean = (tokens * top_k + experts - 1) / experts;
     const int tile_rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
-    const bool x_ok = ((uintptr_t)x & 15) == 0 && d % 8 == 0 && (tokens == 1 || ldx % 8 == 0);
+    // A few tokens: no plan, no slots, one tile per chosen expert.
+    const bool stream = tokens <= 8 && tokens * top_k <= STREAM_PAIRS && stream_x_bytes(tokens, d) <= STREAM_X_BYTES &&
+                        stream_x_bytes(tokens * top_k, f) <= STREAM_X_BYTES;
     // Up to 16 tokens per tile the product gathers x's rows itself (TMA, four
     // rows an instruction, ~20 cycles a row): no launch and no copy. Longer
     // tiles would wait for those rows, and x is spread over the slots first.
     const bool gather = x_ok && tile_rows == 16;
-    const T *w_src[2] = {w_in, w_out};
-    const size_t w_rows[2] = {experts * (gated ? 2 : 1) * f, experts * d}, w_k[2] = {d, f};
-    bool pad[2];
-    size_t off = 0, o_w[2] = {0, 0};
+    size_t off = 0;
     auto take = [&](size_t bytes) {
         const size_t at = off;
         off += Staging::align_up(bytes);
         return at;
     };
+    // Weights whose rows TMA and 128-bit loads cannot read are copied first: all
+    // of them, or, for a few pairs, the named experts'.
+    const T *w_src[2] = {w_in, w_out};
+    const size_t w_er[2] = {(gated ? 2 : 1) * f, d}, w_k[2] = {d, f};
+    bool pad[2];
+    size_t o_w[2] = {0, 0};
     for (int i = 0; i < 2; i++) {
-        pad[i] = !rows16_ok(w_src[i], w_k[i], w_rows[i]);
-        if (pad[i]) o_w[i] = take(w_rows[i] * up8(w_k[i]) * 2);
+        pad[i] = !rows16_ok(w_src[i], w_k[i], experts * w_er[i]);
+        if (pad[i]) o_w[i] = take(experts * w_er[i] * up8(w_k[i]) * 2);
     }
     const size_t per_token = top_k * (ldh * 2 + ldp * 4 + (gather ? 0 : lds * 2) + 8);
     size_t chunk = EXPERTS_WS_BYTES / per_token;
@@ -486,22 +470,68 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
     if (chunk > tokens) chunk = tokens;
     const size_t max_pairs = chunk * top_k;
     const size_t max_tiles = max_pairs / tile_rows + (max_pairs < experts ? max_pairs : experts);
-    const size_t o_pos = take(max_pairs * 4), o_tok = take(gather ? max_pairs * 4 : 0),
-                 o_tiles = take(max_tiles * sizeof(Tile16)), o_n = take(4),
-                 o_x = take(gather ? 0 : max_pairs * lds * 2), o_h = take(max_pairs * ldh * 2),
-                 o_p = take(max_pairs * ldp * 4);
+    size_t o_pos = 0, o_tok = 0, o_tiles = 0, o_n = 0, o_x = 0, o_h, o_p = 0;
+    if (stream) {
+        if (!x_ok) o_x = take(tokens * lds * 2);
+        o_h = take((tokens * top_k < experts ? tokens * top_k : experts) * 8 * ldh * 2);
+    } else {
+        o_pos = take(max_pairs * 4);
+        o_tok = take(gather ? max_pairs * 4 : 0);
+        o_tiles = take(max_tiles * sizeof(Tile16));
+        o_n = take(4);
+        o_x = take(gather ? 0 : max_pairs * lds * 2);
+        o_h = take(max_pairs * ldh * 2);
+        o_p = take(max_pairs * ldp * 4);
+    }
     int st = ensure_ws(ctx, off);
     if (st) return st;
     const void *w_use[2];
     size_t w_ld[2];
-    PadJob job[2];
+    PadJob job[3];
     for (int i = 0; i < 2; i++) {
         w_use[i] = pad[i] ? (const void *)(ctx->ws + o_w[i]) : (const void *)w_src[i];
         w_ld[i] = pad[i] ? up8(w_k[i]) : w_k[i];
-        if (pad[i]) job[i] = PadJob{w_src[i], w_k[i], w_rows[i], w_k[i], ctx->ws + o_w[i]};
+        if (!pad[i]) continue;
+        job[i] = PadJob{w_src[i], w_k[i], experts * w_er[i], w_k[i], ctx->ws + o_w[i], nullptr, 0, w_er[i]};
+        if (tokens * top_k <= 32) {
+            job[i].ids = ids;
+            job[i].pairs = (int)(tokens * top_k);
+        }
     }
-    st = launch_pad_rows16(ctx, job[0], job[1]);
+    if (stream && !x_ok) job[2] = PadJob{x, ldx, tokens, d, ctx->ws + o_x, nullptr, 0, 1};
+    st = launch_pad_rows16(ctx, job[0], job[1], job[2]);
     if (st) return st;
+    Gemm16 g;
+    g.w = w_use[0];
+    g.ldw = w_ld[0];
+    g.w_expert = w_er[0] * w_ld[0];
+    g.n = (int)f;
+    g.k = (int)d;
+    g.experts = (int)experts;
+    g.act = act;
+    g.gated = gated;
+    g.y = ctx->ws + o_h;
+    g.ldy = ldh;
+    Gemm16 o;
+    o.x = g.y;
+    o.ldx = ldh;
+    o.w = w_use[1];
+    o.ldw = w_ld[1];
+    o.w_expert = w_er[1] * w_ld[1];
+    o.n = (int)d;
+    o.k = (int)f;
+    o.experts = (int)experts;
+    if (stream) {
+        g.x = x_ok ? (const void *)x : (const void *)(ctx->ws + o_x);
+        g.ldx = x_ok ? ldx : lds;
+        g.x_rows = (int)tokens;
+        o.x_rows = 8;
+        o.residual = residual;
+        o.ldr = ldr;
+        o.y = y;
+        o.ldy = ldy;
+        return launch_experts_stream(ctx, dtype, g, o, ids, weights, (int)(tokens * top_k), (int)top_k);
+    }
     int *pos = (int *)(ctx->ws + o_pos), *tok = gather ? (int *)(ctx->ws + o_tok) : nullptr;
     int *n_tiles = (int *)(ctx->ws + o_n);
     Tile16 *tiles = (Tile16 *)(ctx->ws + o_tiles);
@@ -549,46 +579,21 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
             st = after_launch(ctx, "experts_spread");
             if (st) return st;
         }
-        Gemm16 g;
         g.x = gather ? (const void *)xt : (const void *)(ctx->ws + o_x);
         g.ldx = gather ? ldx : lds;
         g.x_rows = (int)(gather ? tn : pairs);
-        g.w = w_use[0];
-        g.ldw = w_ld[0];
-        g.w_expert = (gated ? 2 : 1) * f * w_ld[0];
-        g.rows = (int)pairs;
-        g.n = (int)f;
-        g.k = (int)d;
-        g.experts = (int)experts;
         g.row_token = tok;
-        g.tiles = tiles;
-        g.n_tiles = n_tiles;
-        g.max_tiles = (int)(pairs / tile_rows + (pairs < experts ? pairs : experts));
-        g.tile_rows = tile_rows;
-        g.act = act;
-        g.gated = gated;
-        g.y = ctx->ws + o_h;
-        g.ldy = ldh;
-        st = launch_gemm16(ctx, dtype, g);
-        if (st) return st;
-        Gemm16 o;
-        o.x = g.y;
-        o.ldx = ldh;
         o.x_rows = (int)pairs;
-        o.w = w_use[1];
-        o.ldw = w_ld[1];
-        o.w_expert = d * w_ld[1];
-        o.rows = (int)pairs;
-        o.n = (int)d;
-        o.k = (int)f;
-        o.experts = (int)experts;
-        o.tiles = tiles;
-        o.n_tiles = n_tiles;
-        o.max_tiles = g.max_tiles;
-        o.tile_rows = tile_rows;
         o.y = p;
         o.ldy = ldp;
         o.y_f32 = true;
+        g.rows = o.rows = (int)pairs;
+        g.tiles = o.tiles = tiles;
+        g.n_tiles = o.n_tiles = n_tiles;
+        g.max_tiles = o.max_tiles = (int)(pairs / tile_rows + (pairs < experts ? pairs : experts));
+        g.tile_rows = o.tile_rows = tile_rows;
+        st = launch_gemm16(ctx, dtype, g);
+        if (st) return st;
         st = launch_gemm16(ctx, dtype, o);
         if (st) return st;
         const T *rt = residual ? residual + t0 * ldr : nullptr;

@@ -50,7 +50,7 @@ struct Gemm16 {
 // must pass rows16_ok (the copies below make them).
 int launch_gemm16(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g);
 
-// The kernels of a few tokens, for operands of any alignment: a dense product of
+// The kernels of a few tokens, for operands like launch_gemm16's: a dense product of
 // up to STREAM_TOKENS rows, and both of the experts' products of up to
 // STREAM_PAIRS (token, choice) pairs of up to 8 tokens. `in` reads the tokens'
 // rows and writes [tile][8][ldy], one tile per distinct expert; `out` reads
@@ -71,13 +71,17 @@ inline bool rows16_ok(const void *p, size_t ld, size_t rows) {
     return ((uintptr_t)p & 15) == 0 && (rows <= 1 || ld % 8 == 0);
 }
 // dst [rows][k rounded up to a multiple of 8, at least 8] = src [rows][k],
-// zero-filled; two of them in one launch
+// zero-filled; three of them in one launch. With ids only the rows of the experts
+// that they name are copied (up to 32 pairs, expert_rows rows an expert).
 struct PadJob {
     const void *src = nullptr;
     size_t ld = 0, rows = 0, k = 0;
     void *dst = nullptr;
+    const int *ids = nullptr;
+    int pairs = 0;
+    size_t expert_rows = 1;
 };
-int launch_pad_rows16(tpt_cuda_ctx *ctx, const PadJob &a, const PadJob &b);
+int launch_pad_rows16(tpt_cuda_ctx *ctx, const PadJob &a, const PadJob &b, const PadJob &c);
 
 #ifdef __CUDACC__
 

@@ -58,34 +58,20 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Eight 16-bit values from p, of which the first n exist (the rest are 0): one
-// 128-bit load, or by single values where rows do not start on 16 bytes.
-// STREAM: read once, not kept in L1.
-template <bool AL16, bool STREAM>
-__device__ __forceinline__ uint4 load8(const uint16_t *p, int n) {
+// Eight weights where `in` holds (0 elsewhere), read once and not kept in L1
+__device__ __forceinline__ uint4 load8(const uint16_t *p, bool in) {
     uint4 v = make_uint4(0, 0, 0, 0);
-    if constexpr (AL16) {
-        if (n > 0) {  // n is 8 or none: k is a multiple of 8
-            if constexpr (STREAM)
-                asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                             : "l"(p));
-            else
-                v = *reinterpret_cast<const uint4 *>(p);
-        }
-    } else {
-        uint32_t e[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) e[i] = i < n ? (uint32_t)p[i] : 0u;
-        v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-    }
+    if (in)
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "l"(p));
     return v;
 }
 
 // GATED: y = act(W x) * (W2 x). SUM: y[token] = sum over the experts of
 // weight * W_e x_e, x the tiles' rows [tile][token]; otherwise each tile's
 // products go to y's rows [tile][token] (dense: one tile). Up to 8 tokens.
-template <typename T, typename TY, bool GATED, bool SUM, bool AL16>
+template <typename T, typename TY, bool GATED, bool SUM>
 __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant__ StreamArgs a) {
     constexpr int H = GATED ? 2 : 1;
     constexpr int DEPTH = GATED ? 2 : 4;  // steps in flight: 16 loads of 16 bytes a thread
@@ -101,11 +87,11 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
     extern __shared__ __align__(16) uint8_t xs[];
     const uint16_t *w = static_cast<const uint16_t *>(a.w);
     const uint16_t *x = static_cast<const uint16_t *>(a.x);
-    if (AL16 && !a.ids) {
+    if (!a.ids) {
         // a dense layer's rows start towards the L2 while the kernel before it ends
         const int r0 = (int)((long long)a.n * blockIdx.x / gridDim.x), r1 = (int)((long long)a.n * (blockIdx.x + 1) / gridDim.x);
         for (int r = r0 + (int)threadIdx.x; r < r1; r += ST_T)
-            prefetch_l2_bulk(w + (size_t)r * a.ldw, (uint32_t)a.k * 2);
+            prefetch_l2_bulk(w + (size_t)r * a.ldw, (uint32_t)(a.k & ~7) * 2);
     }
     pdl_wait();
     pdl_trigger();
@@ -154,24 +140,17 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
     const int pieces = kch * (ST_CHUNK / 8);  // of 16 bytes, a row
     for (int r = 0; r < x_rows; r++) {
         const uint16_t *src = x + (size_t)(SUM ? slot_row[r] : r) * a.ldx;
-        if constexpr (AL16) {
-            for (int i = threadIdx.x; i < pieces; i += ST_T) {  // all in flight together
-                const bool in = i * 8 < a.k;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(xs) + r * xld + i * 16),
-                             "l"(src + (in ? i * 8 : 0)), "r"(in ? 16 : 0)
-                             : "memory");
-            }
-        } else {
-#pragma unroll 4
-            for (int i = threadIdx.x; i < pieces; i += ST_T)
-                *reinterpret_cast<uint4 *>(xs + (size_t)r * xld + i * 16) =
-                    load8<false, false>(src + i * 8, min(a.k - i * 8, 8));
+        for (int i = threadIdx.x; i < pieces; i += ST_T) {  // all in flight together
+            const int n = min(max(a.k - i * 8, 0), 8);  // values of this piece
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(xs) + r * xld + i * 16),
+                         "l"(src + (n ? i * 8 : 0)), "r"(n * 2)
+                         : "memory");
         }
     }
     bool staged = false;  // whether the warp has waited for them
     auto wait_staged = [&]() {
         if (staged) return;
-        if (AL16) asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
         staged = true;
     };
@@ -202,7 +181,7 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
             const uint8_t *xp = xs + (size_t)(SUM ? tile_slot[tile] + __popc(used & ((1 << g) - 1)) : g) * xld + 16 * t;
             for (int kc = first; kc < last; kc += DEPTH) {
                 uint4 buf[DEPTH][4 * H];
-                if (AL16 && kc + DEPTH <= last && (kc + DEPTH) * ST_CHUNK <= a.k) {
+                if (kc + DEPTH <= last && (kc + DEPTH) * ST_CHUNK <= a.k) {
 #pragma unroll
                     for (int d = 0; d < DEPTH; d++)
 #pragma unroll
@@ -210,8 +189,8 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
 #pragma unroll
                             for (int s = 0; s < 2; s++) {
                                 const size_t o = h * half + (size_t)(kc + d) * ST_CHUNK + 32 * s;
-                                buf[d][h * 4 + s] = load8<true, true>(p0 + o, row0 ? 8 : 0);
-                                buf[d][h * 4 + 2 + s] = load8<true, true>(p1 + o, row1 ? 8 : 0);
+                                buf[d][h * 4 + s] = load8(p0 + o, row0);
+                                buf[d][h * 4 + 2 + s] = load8(p1 + o, row1);
                             }
                 } else {
 #pragma unroll
@@ -221,10 +200,10 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
 #pragma unroll
                             for (int s = 0; s < 2; s++) {
                                 const int k0 = (kc + d) * ST_CHUNK + 32 * s;
-                                const int left = kc + d < last ? min(a.k - k0 - 8 * t, 8) : 0;
+                                const bool in = kc + d < last && k0 + 8 * t < a.k;
                                 const size_t o = h * half + (size_t)k0;
-                                buf[d][h * 4 + s] = load8<AL16, true>(p0 + o, row0 ? left : 0);
-                                buf[d][h * 4 + 2 + s] = load8<AL16, true>(p1 + o, row1 ? left : 0);
+                                buf[d][h * 4 + s] = load8(p0 + o, row0 && in);
+                                buf[d][h * 4 + 2 + s] = load8(p1 + o, row1 && in);
                             }
                 }
                 wait_staged();
@@ -281,9 +260,9 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
     }
 }
 
-template <typename T, typename TY, bool GATED, bool SUM, bool AL16>
+template <typename T, typename TY, bool GATED, bool SUM>
 int launch(tpt_cuda_ctx *ctx, const StreamArgs &a, long long rows, int x_rows) {
-    auto kern = k_gemm16_stream<T, TY, GATED, SUM, AL16>;
+    auto kern = k_gemm16_stream<T, TY, GATED, SUM>;
     static bool done[64] = {};
     const int dev = ctx->device & 63;
     if (!done[dev]) {
@@ -317,19 +296,14 @@ StreamArgs base_args(tpt_cuda_ctx *ctx, const Gemm16 &g) {
 }
 
 template <typename T>
-int dense_typed(tpt_cuda_ctx *ctx, const Gemm16 &g, bool al16) {
+int dense_typed(tpt_cuda_ctx *ctx, const Gemm16 &g) {
     const StreamArgs a = base_args(ctx, g);
-    auto go = [&](auto ty) {
-        using TY = decltype(ty);
-        return al16 ? launch<T, TY, false, false, true>(ctx, a, g.n, g.rows)
-                    : launch<T, TY, false, false, false>(ctx, a, g.n, g.rows);
-    };
-    return g.y_f32 ? go(float()) : go(T());
+    return g.y_f32 ? launch<T, float, false, false>(ctx, a, g.n, g.rows) : launch<T, T, false, false>(ctx, a, g.n, g.rows);
 }
 
 template <typename T>
 int experts_typed(tpt_cuda_ctx *ctx, const Gemm16 &in, const Gemm16 &out, const int *ids, const float *weights,
-                  int pairs, int top_k, bool al16) {
+                  int pairs, int top_k) {
     StreamArgs a = base_args(ctx, in), b = base_args(ctx, out);
     a.ids = b.ids = ids;
     a.weights = b.weights = weights;
@@ -338,35 +312,21 @@ int experts_typed(tpt_cuda_ctx *ctx, const Gemm16 &in, const Gemm16 &out, const 
     a.experts = b.experts = in.experts;
     b.tokens = a.tokens;
     const long long rows = (long long)in.n * (pairs < in.experts ? pairs : in.experts);
-    int st;
-    if (in.gated)
-        st = al16 ? launch<T, T, true, false, true>(ctx, a, rows, a.tokens)
-                  : launch<T, T, true, false, false>(ctx, a, rows, a.tokens);
-    else
-        st = al16 ? launch<T, T, false, false, true>(ctx, a, rows, a.tokens)
-                  : launch<T, T, false, false, false>(ctx, a, rows, a.tokens);
-    if (st) return st;
-    return al16 ? launch<T, T, false, true, true>(ctx, b, out.n, pairs)
-                : launch<T, T, false, true, false>(ctx, b, out.n, pairs);
-}
-
-bool all_aligned(const Gemm16 &g) {
-    return g.k % 8 == 0 && rows16_ok(g.x, g.ldx, (size_t)g.x_rows) && rows16_ok(g.w, g.ldw, 2) &&
-           (g.experts <= 1 || g.w_expert % 8 == 0);
+    const int st = in.gated ? launch<T, T, true, false>(ctx, a, rows, a.tokens)
+                            : launch<T, T, false, false>(ctx, a, rows, a.tokens);
+    return st ? st : launch<T, T, false, true>(ctx, b, out.n, pairs);
 }
 
 }  // namespace
 
 int launch_gemm16_stream(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
-    const bool al = all_aligned(g);
-    return dtype == TPT_DT_BF16 ? dense_typed<__nv_bfloat16>(ctx, g, al) : dense_typed<__half>(ctx, g, al);
+    return dtype == TPT_DT_BF16 ? dense_typed<__nv_bfloat16>(ctx, g) : dense_typed<__half>(ctx, g);
 }
 
 int launch_experts_stream(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &in, const Gemm16 &out, const int *ids,
                           const float *weights, int pairs, int top_k) {
-    const bool al = all_aligned(in) && all_aligned(out);
-    return dtype == TPT_DT_BF16 ? experts_typed<__nv_bfloat16>(ctx, in, out, ids, weights, pairs, top_k, al)
-                                : experts_typed<__half>(ctx, in, out, ids, weights, pairs, top_k, al);
+    return dtype == TPT_DT_BF16 ? experts_typed<__nv_bfloat16>(ctx, in, out, ids, weights, pairs, top_k)
+                                : experts_typed<__half>(ctx, in, out, ids, weights, pairs, top_k);
 }
 
 }  // namespace tpt
