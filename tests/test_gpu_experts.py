@@ -88,6 +88,32 @@ def test_route_groups(cuda, e, groups, kept, top, k, score):
     run_route(cuda, grid_logits(40, e, e + groups), k, score, bias, groups, kept, top, True, 2.5)
 
 
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("e,k,groups,kept,top", [(1, 1, 1, 1, 1), (7, 4, 1, 1, 1), (31, 8, 1, 1, 1), (32, 5, 1, 1, 1),
+                                                 (60, 4, 1, 1, 1), (128, 8, 1, 1, 1), (300, 6, 1, 1, 1),
+                                                 (1024, 8, 1, 1, 1), (256, 8, 8, 4, 2), (64, 3, 32, 7, 2),
+                                                 (60, 8, 5, 2, 1), (765, 8, 17, 3, 2), (1020, 7, 17, 5, 2),
+                                                 (200, 8, 2, 1, 1), (12, 4, 4, 1, 2)])
+def test_route_many_tokens(cuda, e, k, groups, kept, top, ty):
+    """Enough tokens for the kernel whose warps take several: every lane layout, with ties, masks and empty rows."""
+    k = min(k, kept * (e // groups))
+    l = grid_logits(601, e, e + groups, ty)
+    l[5] = -np.inf
+    l[6, e // 2:] = float("nan")
+    l[600, : e // 3] = -np.inf
+    mask = np.ones(601, np.uint8)
+    mask[[3, 77, 599]] = 0
+    rng = np.random.default_rng(e)
+    for score, bias in (("softmax", None), ("sigmoid", (rng.integers(-8, 9, e) / 4).astype(np.float32))):
+        run_route(cuda, l, k, score, bias, groups, kept, top, e % 2 == 0, 2.5, mask)
+
+
+@pytest.mark.parametrize("t", [1, 591, 592, 700])
+def test_route_strided_many_tokens(cuda, t):
+    run_route(cuda, grid_logits(t, 80, 9, "bf16")[:, 5:75], 6)
+    run_route(cuda, grid_logits(t, 80, 9, "f32")[:, 4:76], 3, groups=2, kept=1)
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("groups,kept", [(1, 1), (4, 2)])
 def test_route_masked_experts_and_tokens(cuda, score, groups, kept):

@@ -20,7 +20,7 @@ namespace {
 
 // ------------------------------------------------------------------ routing
 
-constexpr int ROUTE_WARPS = 4;
+constexpr int ROUTE_WARPS = 8;
 
 // A total order of floats as unsigned integers; NaN does not occur.
 __device__ __forceinline__ unsigned order_key(float v) {
@@ -77,7 +77,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32)
     k_route_experts(const T *__restrict__ logits, size_t ld, int tokens, int experts, int softmax,
                     const float *__restrict__ bias, int groups, int groups_kept, int group_top, int lanes, int vec,
-                    int top_k, int renormalise, float scale, const uint8_t *__restrict__ mask, int *__restrict__ ids,
+                    int bias_vec, int top_k, int renormalise, float scale, const uint8_t *__restrict__ mask, int *__restrict__ ids,
                     float *__restrict__ weights) {
     pdl_wait();
     pdl_trigger();
@@ -115,17 +115,19 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32)
             for (int i = 0; i < V; i++) c[i] = c[i] > NEG ? sigmoid_score(c[i]) : NEG;
         }
         if (bias) {
+            float bv[V];
+            load_logits<float, V>(bias + e0, bias_vec, n, bv);
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                const float b = c[i] + (i < n ? __ldg(bias + e0 + i) : 0.0f);
-                c[i] = c[i] > NEG && b > NEG ? b : NEG;  // a NaN or -inf bias switches the expert off
-            }
+            for (int i = 0; i < V; i++) bv[i] = c[i] + bv[i];
+#pragma unroll
+            for (int i = 0; i < V; i++) c[i] = c[i] > NEG && bv[i] > NEG ? bv[i] : NEG;  // a NaN or -inf bias: off, too
         }
         // This lane's best two, the lower index first among equals; `gone` marks
         // the ones already chosen.
         float b1, b2;
         int i1, i2;
-        unsigned long long gone = 0;
+        using Bits = typename std::conditional<(V > 32), unsigned long long, unsigned>::type;
+        Bits gone = 0;
         auto scan = [&]() {
             b1 = b2 = NEG;
             i1 = i2 = 0;
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32)
             }
             if (better >= groups_kept) {  // nothing of this lane can be chosen
                 b1 = b2 = NEG;
-                gone = ~0ull;
+                gone = ~(Bits)0;
             }
         }
         int cached = 2;  // how many of (b1, b2) stand
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32)
             const int e = __shfl_sync(0xffffffffu, e0 + i1, owner);
             if (lane == j) id_mine = e;
             if (lane == owner) {
-                gone |= 1ull << i1;
+                gone |= (Bits)1 << i1;
                 b1 = b2;
                 i1 = i2;
                 cached--;
@@ -208,9 +210,11 @@ void launch_route(tpt_cuda_ctx *ctx, const void *logits, size_t ld, int tokens, 
     while (v < need) v *= 2;
     const size_t word = v * sizeof(T) < 16 ? v * sizeof(T) : 16;
     const bool vec = per % v == 0 && ((uintptr_t)logits % word) == 0 && (tokens == 1 || ld * sizeof(T) % word == 0);
+    const size_t bword = v * 4 < 16 ? v * 4 : 16;
+    const bool bias_vec = per % v == 0 && ((uintptr_t)bias % bword) == 0;
     auto go = [&](auto kern) {
         launch_pdl(kern, grid, ROUTE_WARPS * 32, 0, ctx->stream, (const T *)logits, ld, tokens, experts,
-                   score == TPT_SCORE_SOFTMAX, bias, groups, groups_kept, group_top, lanes, vec, top_k, renormalise,
+                   score == TPT_SCORE_SOFTMAX, bias, groups, groups_kept, group_top, lanes, vec, bias_vec, top_k, renormalise,
                    scale, mask, ids, weights);
     };
     // groups <= 32 and experts <= 1024: at most 64 experts a lane (17 groups of 60)
