@@ -78,74 +78,88 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
     constexpr int COLS = 8;
     __shared__ float red[2][ST_WARPS][H][ST_ROWS][COLS];
     __shared__ int tile_expert[32];
-    __shared__ float tile_w[SUM ? 32 : 1][8];
-    __shared__ int tile_used[SUM ? 32 : 1];
+    // SUM: per tile the tokens that chose the expert, per tile and token its weight
+    // and its staged row, per staged row its tile * 8 + token
+    __shared__ int tile_used[SUM ? 32 : 1], slot_of[SUM ? 256 : 1], slot_row[SUM ? 32 : 1];
+    __shared__ float tile_w[SUM ? 256 : 1];
+    extern __shared__ __align__(16) uint8_t xs[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    __shared__ int slot_row[SUM ? 32 : 1];  // the staged rows: (tile * 8 + token) of each
-    __shared__ int tile_slot[SUM ? 32 : 1];  // a tile's first
-    extern __shared__ __align__(16) uint8_t xs[];
     const uint16_t *w = static_cast<const uint16_t *>(a.w);
     const uint16_t *x = static_cast<const uint16_t *>(a.x);
+    // this block's equal share of `rows`: rows [first, end) (32-bit: a 64-bit
+    // division is hundreds of cycles)
+    auto share = [](int rows, int &first, int &end) {
+        const int q = rows / (int)gridDim.x, r = rows - q * (int)gridDim.x, b = (int)blockIdx.x;
+        first = b * q + min(b, r);
+        end = first + q + (b < r ? 1 : 0);
+    };
+    int at = 0, end = 0;  // the block's rows; `at` is the first row of its group
+    if (SUM || !a.ids) share(a.n, at, end);
     if (!a.ids) {
         // a dense layer's rows start towards the L2 while the kernel before it ends
-        const int r0 = (int)((long long)a.n * blockIdx.x / gridDim.x), r1 = (int)((long long)a.n * (blockIdx.x + 1) / gridDim.x);
-        for (int r = r0 + (int)threadIdx.x; r < r1; r += ST_T)
+        for (int r = at + (int)threadIdx.x; r < end; r += ST_T)
             prefetch_l2_bulk(w + (size_t)r * a.ldw, (uint32_t)(a.k & ~7) * 2);
     }
+    const int kch = (a.k + ST_CHUNK - 1) / ST_CHUNK;  // steps of one product
     pdl_wait();
     pdl_trigger();
     int n_tiles = 1, x_rows = a.tokens;
     if (a.ids) {
-        // the distinct experts, in the order of their first choice (every warp alike)
+        // lane p is pair p; every warp finds the distinct experts (in the order of
+        // their first choice), the first one writes the tables
         const int id = lane < a.pairs ? __ldcg(a.ids + lane) : -1;
+        const float weight = SUM && lane < a.pairs ? a.weights[lane] : 0.0f;
+        const int tok = lane / a.top_k;
         const bool valid = id >= 0 && id < a.experts;
         if (warp == 0 && id >= a.experts) atomicOr(a.gflags + TPT_FLAG_CHECK, 1u);
+        const unsigned below = (1u << lane) - 1;
         const unsigned same = __match_any_sync(0xffffffffu, valid ? id : -1 - lane);
-        const bool first = valid && __ffs(same) - 1 == lane;
-        const unsigned firsts = __ballot_sync(0xffffffffu, first);
+        const int leader = __ffs(same) - 1;
+        const unsigned firsts = __ballot_sync(0xffffffffu, valid && leader == lane);
         n_tiles = __popc(firsts);
-        const int tile = __popc(firsts & ((1u << lane) - 1));
-        if (warp == 0 && first) tile_expert[tile] = id;
+        const int tile = __popc(firsts & ((1u << leader) - 1));
+        if (warp == 0 && valid && leader == lane) tile_expert[tile] = id;
         if (SUM) {
-            int used = 0;
-            if (first)
-                for (unsigned m = same; m; m &= m - 1) used |= 1 << ((__ffs(m) - 1) / a.top_k);
-            int end = __popc(used);  // inclusive sum over the tiles' rows
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, end, o);
-                if (lane >= o) end += v;
-            }
-            x_rows = __shfl_sync(0xffffffffu, end, 31);
-            if (warp == 0 && first) {
-                // a token that chose the expert twice takes it once, with both weights
-                for (int i = 0; i < 8; i++) tile_w[tile][i] = 0.0f;
-                for (unsigned m = same; m; m &= m - 1) {
-                    const int p = __ffs(m) - 1;
-                    tile_w[tile][p / a.top_k] += a.weights[p];
+            // a token that chose the expert twice takes it once, with both weights
+            const unsigned twin = __match_any_sync(0xffffffffu, valid ? id * 8 + tok : -1 - lane);
+            const bool row = valid && __ffs(twin) - 1 == lane;
+            const unsigned slots = __ballot_sync(0xffffffffu, row);
+            x_rows = __popc(slots);
+            float sum = weight;
+            if (__any_sync(0xffffffffu, valid && __popc(twin) > 1)) {
+                sum = 0.0f;
+                for (int j = 0; j < 32; j++) {
+                    const float v = __shfl_sync(0xffffffffu, weight, j);
+                    if (twin >> j & 1) sum += v;
                 }
+            }
+            if (warp == 0 && row) {
+                const int slot = __popc(slots & below);
+                slot_row[slot] = tile * 8 + tok;
+                slot_of[tile * 8 + tok] = slot;
+                tile_w[tile * 8 + tok] = sum;
+            }
+            if (warp == 0 && valid && leader == lane) {
+                int used = 0;
+                for (unsigned m = same; m; m &= m - 1) used |= 1 << ((__ffs(m) - 1) / a.top_k);
                 tile_used[tile] = used;
-                int at = end - __popc(used);
-                tile_slot[tile] = at;
-                for (int m = used; m; m &= m - 1) slot_row[at++] = tile * 8 + __ffs(m) - 1;
             }
         }
         __syncthreads();
+        if (!SUM) share(n_tiles * a.n, at, end);
     }
-    const int kch = (a.k + ST_CHUNK - 1) / ST_CHUNK;  // steps of one product
     // the tokens' rows, zero past k; 16 bytes more than a multiple of 128 from one
     // to the next, so that eight rows' fragments lie in different banks
     const int xld = kch * ST_CHUNK * 2 + 16;
     const int pieces = kch * (ST_CHUNK / 8);  // of 16 bytes, a row
-    for (int r = 0; r < x_rows; r++) {
+    for (int i = threadIdx.x; i < x_rows * pieces; i += ST_T) {  // all in flight together
+        const int r = i / pieces, c = (i - r * pieces) * 8;
+        const int n = min(max(a.k - c, 0), 8);  // values of this piece
         const uint16_t *src = x + (size_t)(SUM ? slot_row[r] : r) * a.ldx;
-        for (int i = threadIdx.x; i < pieces; i += ST_T) {  // all in flight together
-            const int n = min(max(a.k - i * 8, 0), 8);  // values of this piece
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(xs) + r * xld + i * 16),
-                         "l"(src + (n ? i * 8 : 0)), "r"(n * 2)
-                         : "memory");
-        }
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(xs) + r * xld + c * 2),
+                     "l"(src + (n ? c : 0)), "r"(n * 2)
+                     : "memory");
     }
     bool staged = false;  // whether the warp has waited for them
     auto wait_staged = [&]() {
@@ -155,106 +169,150 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
         staged = true;
     };
 
-    const int total = SUM ? a.n : n_tiles * a.n;
-    const int end = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
     const int chunks = SUM ? kch * n_tiles : kch;  // steps of one output, split over the warps
-    const int c0 = (int)((long long)chunks * warp / ST_WARPS), c1 = (int)((long long)chunks * (warp + 1) / ST_WARPS);
+    const int c0 = chunks * warp / ST_WARPS, c1 = chunks * (warp + 1) / ST_WARPS;
     const size_t half = (size_t)a.n * a.ldw;
-    int rb = 0;
-    // groups of up to 16 rows of one expert's features
-    for (int at = (int)((long long)total * blockIdx.x / gridDim.x), rows; at < end; at += rows) {
-        const int out_tile = SUM ? 0 : at / a.n;
-        const int f = at - out_tile * a.n;
-        const int rem = min(end - at, a.n - f), parts = (rem + ST_ROWS - 1) / ST_ROWS;
-        rows = (rem + parts - 1) / parts;
+    // The warp's walk: groups of up to 16 rows of one expert's features; in a
+    // group, the warp's steps [c0, c1) as segments of one expert's k; in a segment,
+    // rounds of DEPTH steps. A round's loads go out as soon as the one before it
+    // has been consumed, across the ends of segments and groups, so that a group's
+    // sums meet while the next group's weights come.
+    int rows = 0, out_tile = 0, f = 0;
+    int c = c1, tile = 0, kc = 0, last = 0;  // segment of expert `tile`: steps [kc, last) are left
+    const uint16_t *p0 = w;
+    auto segment = [&]() {
+        if (c >= c1) {  // the warp has no step (left) in this group
+            kc = last = 0;
+            return;
+        }
+        tile = SUM ? c / kch : out_tile;
+        kc = SUM ? c - tile * kch : c;
+        last = min(kch, kc + c1 - c);
+        c += last - kc;
+        p0 = w + (a.ids ? (size_t)tile_expert[tile] * a.w_expert : 0) + (size_t)(f + g) * a.ldw + 8 * t;
+    };
+    auto group = [&]() {
+        rows = 0;
+        if (at < end) {
+            out_tile = SUM ? 0 : at / a.n;
+            f = at - out_tile * a.n;
+            const int rem = min(end - at, a.n - f), parts = (rem + ST_ROWS - 1) / ST_ROWS;
+            rows = (rem + parts - 1) / parts;
+            c = c0;
+            segment();
+        } else {
+            kc = last = 0;
+        }
+    };
+    uint4 buf[DEPTH][4 * H];
+    auto fetch = [&]() {
+        if (kc >= last) return;
         const bool row0 = g < rows, row1 = g + 8 < rows;
-        float acc[H][4] = {}, sum[4] = {};
-        for (int c = c0; c < c1;) {
-            const int tile = SUM ? c / kch : out_tile;
-            const int first = SUM ? c - tile * kch : c, last = min(kch, first + c1 - c);  // steps of this expert's k
-            c += last - first;
-            const uint16_t *p0 = w + (a.ids ? (size_t)tile_expert[tile] * a.w_expert : 0) + (size_t)(f + g) * a.ldw + 8 * t;
-            const uint16_t *p1 = p0 + 8 * a.ldw;
-            const int used = SUM ? tile_used[tile] : 0;
-            // this lane's column is token g
-            const bool in = SUM ? (used >> g & 1) != 0 : g < a.tokens;
-            const uint8_t *xp = xs + (size_t)(SUM ? tile_slot[tile] + __popc(used & ((1 << g) - 1)) : g) * xld + 16 * t;
-            for (int kc = first; kc < last; kc += DEPTH) {
-                uint4 buf[DEPTH][4 * H];
-                if (kc + DEPTH <= last && (kc + DEPTH) * ST_CHUNK <= a.k) {
+        const uint16_t *p1 = p0 + 8 * a.ldw;
+        if (kc + DEPTH <= last && (kc + DEPTH) * ST_CHUNK <= a.k) {
 #pragma unroll
-                    for (int d = 0; d < DEPTH; d++)
+            for (int d = 0; d < DEPTH; d++)
 #pragma unroll
-                        for (int h = 0; h < H; h++)
-#pragma unroll
-                            for (int s = 0; s < 2; s++) {
-                                const size_t o = h * half + (size_t)(kc + d) * ST_CHUNK + 32 * s;
-                                buf[d][h * 4 + s] = load8(p0 + o, row0);
-                                buf[d][h * 4 + 2 + s] = load8(p1 + o, row1);
-                            }
-                } else {
-#pragma unroll
-                    for (int d = 0; d < DEPTH; d++)
-#pragma unroll
-                        for (int h = 0; h < H; h++)
-#pragma unroll
-                            for (int s = 0; s < 2; s++) {
-                                const int k0 = (kc + d) * ST_CHUNK + 32 * s;
-                                const bool in = kc + d < last && k0 + 8 * t < a.k;
-                                const size_t o = h * half + (size_t)k0;
-                                buf[d][h * 4 + s] = load8(p0 + o, row0 && in);
-                                buf[d][h * 4 + 2 + s] = load8(p1 + o, row1 && in);
-                            }
-                }
-                wait_staged();
-#pragma unroll
-                for (int d = 0; d < DEPTH; d++) {
-                    if (kc + d >= last) break;
+                for (int h = 0; h < H; h++)
 #pragma unroll
                     for (int s = 0; s < 2; s++) {
-                        uint4 xv = make_uint4(0, 0, 0, 0);
-                        if (in) xv = *reinterpret_cast<const uint4 *>(xp + (kc + d) * (ST_CHUNK * 2) + 64 * s);
+                        const size_t o = h * half + (size_t)(kc + d) * ST_CHUNK + 32 * s;
+                        buf[d][h * 4 + s] = load8(p0 + o, row0);
+                        buf[d][h * 4 + 2 + s] = load8(p1 + o, row1);
+                    }
+        } else {
 #pragma unroll
-                        for (int h = 0; h < H; h++) {
-                            const uint4 lo = buf[d][h * 4 + s], hi = buf[d][h * 4 + 2 + s];
-                            mma16816<T>(acc[h], lo.x, hi.x, lo.y, hi.y, xv.x, xv.y);
-                            mma16816<T>(acc[h], lo.z, hi.z, lo.w, hi.w, xv.z, xv.w);
-                        }
+            for (int d = 0; d < DEPTH; d++)
+#pragma unroll
+                for (int h = 0; h < H; h++)
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        const int k0 = (kc + d) * ST_CHUNK + 32 * s;
+                        const bool in = kc + d < last && k0 + 8 * t < a.k;
+                        const size_t o = h * half + (size_t)k0;
+                        buf[d][h * 4 + s] = load8(p0 + o, row0 && in);
+                        buf[d][h * 4 + 2 + s] = load8(p1 + o, row1 && in);
+                    }
+        }
+    };
+    group();
+    fetch();
+    int rb = 0;
+    while (rows > 0) {
+        const int g_rows = rows, g_f = f, g_tile = out_tile;
+        float acc[H][4] = {}, sum[4] = {};
+        bool more = kc < last;
+        while (more) {
+            // this lane's column is token g
+            const int used = SUM ? tile_used[tile] : 0;
+            const bool in = SUM ? (used >> g & 1) != 0 : g < a.tokens;
+            const uint8_t *xp = xs + (in && SUM ? slot_of[tile * 8 + g] : g) * xld + 16 * t;
+            wait_staged();
+#pragma unroll
+            for (int d = 0; d < DEPTH; d++) {
+                if (kc + d >= last) break;
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    uint4 xv = make_uint4(0, 0, 0, 0);
+                    if (in) xv = *reinterpret_cast<const uint4 *>(xp + (kc + d) * (ST_CHUNK * 2) + 64 * s);
+#pragma unroll
+                    for (int h = 0; h < H; h++) {
+                        const uint4 lo = buf[d][h * 4 + s], hi = buf[d][h * 4 + 2 + s];
+                        mma16816<T>(acc[h], lo.x, hi.x, lo.y, hi.y, xv.x, xv.y);
+                        mma16816<T>(acc[h], lo.z, hi.z, lo.w, hi.w, xv.z, xv.w);
                     }
                 }
             }
-            if constexpr (SUM) {  // the warp's share of this expert's products: weigh it
+            const int weigh = tile;
+            kc += DEPTH;
+            const bool seg_end = kc >= last;
+            if (seg_end) {
+                more = c < c1;
+                if (more) {
+                    segment();
+                } else {
+                    at += rows;
+                    group();
+                }
+            }
+            fetch();
+            if (SUM && seg_end) {  // the warp's share of this expert's products: weigh it
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int tok = 2 * t + (i & 1);
                     // a token without this expert takes nothing of it, not 0 x inf
-                    if (used >> tok & 1) sum[i] = fmaf(tile_w[tile][tok], acc[0][i], sum[i]);
+                    if (used >> tok & 1) sum[i] = fmaf(tile_w[weigh * 8 + tok], acc[0][i], sum[i]);
                     acc[0][i] = 0.0f;
                 }
             }
         }
+        if (c0 >= c1) {  // no share: on to the next group
+            at += rows;
+            group();
+        }
         wait_staged();
 #pragma unroll
         for (int h = 0; h < H; h++)
+#pragma unroll
             for (int i = 0; i < 2; i++)
                 *reinterpret_cast<float2 *>(&red[rb][warp][h][g + 8 * i][2 * t]) =
                     SUM ? make_float2(sum[2 * i], sum[2 * i + 1]) : make_float2(acc[h][2 * i], acc[h][2 * i + 1]);
         __syncthreads();
-        // one output a thread: feature f + r of token o
+        // one output a thread: feature g_f + r of token o
         const int r = threadIdx.x & 15, o = threadIdx.x >> 4;
-        if (o < COLS && o < a.tokens && r < rows) {
+        if (o < COLS && o < a.tokens && r < g_rows) {
             float v[1] = {0.0f}, u = 0.0f;
 #pragma unroll
             for (int i = 0; i < ST_WARPS; i++) {
                 v[0] += red[rb][i][0][r][o];
                 if (GATED) u += red[rb][i][H - 1][r][o];
             }
-            if (a.bias) v[0] += to_f32(static_cast<const T *>(a.bias)[f + r]);
+            if (a.bias) v[0] += to_f32(static_cast<const T *>(a.bias)[g_f + r]);
             act16(v, a.act);
             if (GATED) v[0] *= u;
-            if (a.residual) v[0] += to_f32(static_cast<const TY *>(a.residual)[(size_t)o * a.ldr + f + r]);
-            const size_t row = a.ids && !SUM ? (size_t)out_tile * 8 + o : (size_t)o;
-            static_cast<TY *>(a.y)[row * a.ldy + f + r] = from_f32<TY>(v[0]);
+            if (a.residual) v[0] += to_f32(static_cast<const TY *>(a.residual)[(size_t)o * a.ldr + g_f + r]);
+            const size_t row = a.ids && !SUM ? (size_t)g_tile * 8 + o : (size_t)o;
+            static_cast<TY *>(a.y)[row * a.ldy + g_f + r] = from_f32<TY>(v[0]);
         }
         rb ^= 1;  // the next group's sums go beside these; the barrier after it frees them
     }
