@@ -323,6 +323,33 @@ def test_experts_bad_tokens_stay_apart(cuda, t):
     check(y[keep], *want_experts(x[keep], ids[keep], wts[keep], w_in, w_out, "silu", True, None, "bf16"))
 
 
+@pytest.mark.parametrize("t", [3, 60, 700])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan"), 3e38])
+def test_experts_bad_weights_stay_in_their_features(cuda, bad, t):
+    """An infinity, a NaN or a product at the end of f32's range in one output feature of one expert, with products of
+    very different size beside it: every other feature is right, for all tokens."""
+    import torch
+
+    x, ids, wts, w_in, w_out = expert_inputs(t, 4, 2, 200, 72, "bf16", True)
+    w_out[1, 70, 3] = bad
+    w_out[2, 40:60] *= 1e-20
+    w_out[3] = 0
+    y = torch.empty_like(x)
+    torch.cuda.synchronize()
+    cuda.experts_mlp_dev(x, ids, wts, w_in, w_out, 3, True, None, y)
+    cuda.sync()
+    clean = w_out.clone()
+    clean[1, 70] = 0
+    ref, bound = want_experts(x, ids, wts, w_in, clean, "silu", True, None, "bf16")
+    hit = (ids == 1).any(1)
+    keep = torch.ones(200, dtype=torch.bool, device="cuda")
+    keep[70] = False
+    check(y[:, keep], ref[:, keep], bound[:, keep])
+    check(y[~hit], ref[~hit], bound[~hit])
+    if bad != 3e38:
+        assert not torch.isfinite(y[hit, 70]).any()
+
+
 def test_experts_many_tokens_in_chunks(cuda):
     """More intermediate results than the workspace takes at once."""
     x, ids, wts, w_in, w_out = expert_inputs(17000, 8, 8, 4096, 64, "bf16", True)
