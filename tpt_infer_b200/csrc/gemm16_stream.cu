@@ -102,8 +102,13 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
             prefetch_l2_bulk(w + (size_t)r * a.ldw, (uint32_t)(a.k & ~7) * 2);
     }
     const int kch = (a.k + ST_CHUNK - 1) / ST_CHUNK;  // steps of one product
-    pdl_wait();
-    pdl_trigger();
+    // SUM waits for the kernel before it only where it reads h. That kernel, the
+    // first product of the same call, let this one start after its own wait, so what
+    // earlier kernels wrote (ids, weights, W) is complete; and it writes only h.
+    if (!SUM) {
+        pdl_wait();
+        pdl_trigger();
+    }
     int n_tiles = 1, x_rows = a.tokens;
     if (a.ids) {
         // lane p is pair p; every warp finds the distinct experts (in the order of
@@ -149,26 +154,6 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
         __syncthreads();
         if (!SUM) share(n_tiles * a.n, at, end);
     }
-    // the tokens' rows, zero past k; 16 bytes more than a multiple of 128 from one
-    // to the next, so that eight rows' fragments lie in different banks
-    const int xld = kch * ST_CHUNK * 2 + 16;
-    const int pieces = kch * (ST_CHUNK / 8);  // of 16 bytes, a row
-    for (int i = threadIdx.x; i < x_rows * pieces; i += ST_T) {  // all in flight together
-        const int r = i / pieces, c = (i - r * pieces) * 8;
-        const int n = min(max(a.k - c, 0), 8);  // values of this piece
-        const uint16_t *src = x + (size_t)(SUM ? slot_row[r] : r) * a.ldx;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(xs) + r * xld + c * 2),
-                     "l"(src + (n ? c : 0)), "r"(n * 2)
-                     : "memory");
-    }
-    bool staged = false;  // whether the warp has waited for them
-    auto wait_staged = [&]() {
-        if (staged) return;
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();
-        staged = true;
-    };
-
     const int chunks = SUM ? kch * n_tiles : kch;  // steps of one output, split over the warps
     const int c0 = chunks * warp / ST_WARPS, c1 = chunks * (warp + 1) / ST_WARPS;
     const size_t half = (size_t)a.n * a.ldw;
@@ -236,7 +221,32 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
         }
     };
     group();
-    fetch();
+    if (SUM) {
+        fetch();
+        pdl_wait();
+        pdl_trigger();
+    }
+    // the tokens' rows, zero past k; 16 bytes more than a multiple of 128 from one
+    // to the next, so that eight rows' fragments lie in different banks
+    const int xld = kch * ST_CHUNK * 2 + 16;
+    const int pieces = kch * (ST_CHUNK / 8);  // of 16 bytes, a row
+    for (int i = threadIdx.x; i < x_rows * pieces; i += ST_T) {  // all in flight together
+        const int r = i / pieces, c = (i - r * pieces) * 8;
+        const int n = min(max(a.k - c, 0), 8);  // values of this piece
+        const uint16_t *src = x + (size_t)(SUM ? slot_row[r] : r) * a.ldx;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(xs) + r * xld + c * 2),
+                     "l"(src + (n ? c : 0)), "r"(n * 2)
+                     : "memory");
+    }
+    bool staged = false;  // whether the warp has waited for them
+    auto wait_staged = [&]() {
+        if (staged) return;
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();
+        staged = true;
+    };
+
+    if (!SUM) fetch();
     int rb = 0;
     while (rows > 0) {
         const int g_rows = rows, g_f = f, g_tile = out_tile;
