@@ -240,19 +240,19 @@ void launch_route(tpt_cuda_ctx *ctx, const void *logits, size_t ld, int tokens, 
 // expert), row_token[slot] its token (null: not wanted); tiles lists each
 // expert's slots in runs of at most tile_rows, an expert's runs of equal
 // length up to the step that the product kernels count columns in.
-// One cluster of CL blocks: each counts its share of the pairs in shared
-// memory, the blocks add one another's counts, and each places its share.
-constexpr int PLAN_T = 1024;
+// One cluster of eight blocks: each counts its share of the pairs in shared
+// memory, the blocks add one another's counts, and each places its share (65536
+// pairs of 128 experts: 9 us).
+constexpr int PLAN_T = 1024, CL = 8;
 
-template <int CL>
-__global__ void __launch_bounds__(PLAN_T)
+__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(PLAN_T)
     k_experts_plan(const int *__restrict__ ids, int pairs, int top_k, int experts, int tile_rows, int step, int *pos,
                    int *row_token, Tile16 *tiles, int *n_tiles, unsigned *gflags) {
     extern __shared__ int plan_smem[];
     int *count = plan_smem, *first = plan_smem + experts;
     __shared__ int warp_slots[PLAN_T / 32], warp_tiles[PLAN_T / 32];
     __shared__ int run_slots, run_tiles;
-    const int rank = CL > 1 ? (int)tc::cluster_rank() : 0;
+    const int rank = (int)tc::cluster_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int e = threadIdx.x; e < experts; e += PLAN_T) count[e] = 0;
     if (threadIdx.x == 0) run_slots = run_tiles = 0;
@@ -269,27 +269,21 @@ __global__ void __launch_bounds__(PLAN_T)
             atomicAdd(&count[e], 1);
     }
     if (bad) atomicOr(gflags + TPT_FLAG_CHECK, 1u);
-    if (CL > 1)
-        tc::cluster_sync();
-    else
-        __syncthreads();
+    __syncwarp();
+    tc::cluster_sync();
     // first[e]: the first slot of this block's pairs of expert e. Exclusive sums
     // over the experts, PLAN_T at a time; block 0 writes the tiles on the way.
     for (int e0 = 0; e0 < experts; e0 += PLAN_T) {
         const int e = e0 + threadIdx.x;
         int total = 0, before = 0;
         if (e < experts) {
-            if (CL > 1) {
-                const uint32_t at = tc::smem_u32(count + e);
+            const uint32_t at = tc::smem_u32(count + e);
 #pragma unroll
-                for (int r = 0; r < CL; r++) {
-                    int v;
-                    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(tc::map_to_rank(at, (uint32_t)r)) : "memory");
-                    if (r < rank) before += v;
-                    total += v;
-                }
-            } else {
-                total = count[e];
+            for (int r = 0; r < CL; r++) {
+                int v;
+                asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(tc::map_to_rank(at, (uint32_t)r)) : "memory");
+                if (r < rank) before += v;
+                total += v;
             }
         }
         const int nt = (total + tile_rows - 1) / tile_rows;
@@ -341,7 +335,8 @@ __global__ void __launch_bounds__(PLAN_T)
         }
         pos[i] = slot;
     }
-    if (CL > 1) tc::cluster_sync();  // the counts are read by the other blocks
+    __syncwarp();
+    tc::cluster_sync();  // the counts are read by the other blocks
 }
 
 // xs[pos[t, j], :] = x[t, :] for every choice j: each token's row is read once
@@ -441,18 +436,21 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
     auto up8 = [](size_t v) { return (v + 7) / 8 * 8; };
     const size_t ldh = up8(f), lds = up8(d), ldp = (d + 3) / 4 * 4;  // rows start on 16 bytes
     const bool x_ok = d % 8 == 0 && rows16_ok(x, ldx, tokens);
-    // Tokens per tile of the products: what an expert gets on average, up to the
-    // pair kernel's 256 columns.
+    // Tokens per tile of the products, by what an expert gets on average (experts
+    // draw unevenly: many get far more). 128 experts of 2048 x 768, 8 chosen, us with
+    // tiles of 16 / 32 / 256: 64 tokens (mean 4) 178 / 182 / 193, 256 tokens (16) 220 /
+    // 210 / 225, 512 tokens (32) 305 / 239 / 233, 2048 tokens (128) 862 / 494 / 311.
     const size_t mean = (tokens * top_k + experts - 1) / experts;
-    const int tile_rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
+    const int tile_rows = mean <= 10 ? 16 : mean <= 24 ? 32 : 256;
     // A few tokens: no plan, no slots, one tile per chosen expert (128 experts of
     // 2048 x 768, 8 chosen: 1 token 24 us against 29, 4 tokens 57 against 58; 8 tokens of
     // 64 experts, 4 chosen: 30 against 24).
     const bool stream = tokens <= 4 && tokens * top_k <= STREAM_PAIRS && stream_x_bytes(tokens, d) <= STREAM_X_BYTES &&
                         stream_x_bytes(tokens * top_k, f) <= STREAM_X_BYTES;
-    // Up to 16 tokens per tile the product gathers x's rows itself (TMA, four
-    // rows an instruction, ~20 cycles a row): no launch and no copy. Longer
-    // tiles would wait for those rows, and x is spread over the slots first.
+    // With tiles of 16 tokens the product gathers x's rows itself (TMA, four rows
+    // an instruction, ~20 cycles a row): no launch and no copy. Longer tiles would
+    // wait for those rows (8192 tokens: 1192 us gathered, 49 + 355 us spread), and x is
+    // spread over the slots first.
     const bool gather = x_ok && tile_rows == 16;
     size_t off = 0;
     auto take = [&](size_t bytes) {
@@ -546,30 +544,8 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
         const size_t tn = tokens - t0 < chunk ? tokens - t0 : chunk;
         const size_t pairs = tn * top_k;
         const T *xt = x + t0 * ldx;
-        // one block places up to 8192 pairs in about the time that a cluster of
-        // eight takes to meet
-        auto plan = [&](auto kern, int cl) {
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(cl);
-            cfg.blockDim = dim3(PLAN_T);
-            cfg.dynamicSmemBytes = experts * 8;
-            cfg.stream = ctx->stream;
-            cudaLaunchAttribute at[2];
-            at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-            at[0].val.programmaticStreamSerializationAllowed = 1;
-            at[1].id = cudaLaunchAttributeClusterDimension;
-            at[1].val.clusterDim.x = cl;
-            at[1].val.clusterDim.y = 1;
-            at[1].val.clusterDim.z = 1;
-            cfg.attrs = at;
-            cfg.numAttrs = cl > 1 ? 2 : 1;
-            (void)cudaLaunchKernelEx(&cfg, kern, ids + t0 * top_k, (int)pairs, (int)top_k, (int)experts, tile_rows,
-                                     tile_rows == 256 ? 32 : 16, pos, tok, tiles, n_tiles, ctx->d_flags);
-        };
-        if (pairs <= 8192)
-            plan(k_experts_plan<1>, 1);
-        else
-            plan(k_experts_plan<8>, 8);
+        launch_pdl(k_experts_plan, CL, PLAN_T, experts * 8, ctx->stream, ids + t0 * top_k, (int)pairs, (int)top_k,
+                   (int)experts, tile_rows, tile_rows == 256 ? 32 : 16, pos, tok, tiles, n_tiles, ctx->d_flags);
         st = after_launch(ctx, "experts_plan");
         if (st) return st;
         if (!gather) {
