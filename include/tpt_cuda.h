@@ -421,6 +421,8 @@ int tpt_cuda_plan_run_batches(tpt_cuda_plan *plan, const int *in_ids, const floa
  * limits, TPT_SHAPE_MISMATCH for a stride shorter than its row, TPT_INVALID
  * for anything else (null or misaligned pointers, unknown enum values). */
 
+#define TPT_LINEAR_MAX 0x3fffff00 /* m, n, k; tokens, d, f */
+
 /* y[m, n] = act(x[m, k] w[n, k]^T + bias[n]) + residual[m, n]. bias (of the
  * operands' type) and residual (of y's type) may be NULL; y_dtype is the
  * operands' type or TPT_DT_F32. k = 0 gives act(bias) + residual. */
@@ -436,10 +438,10 @@ int tpt_cuda_linear_dev(tpt_cuda_ctx *ctx, int dtype, const void *x, size_t ldx,
  * the groups_kept best groups (ties: lowest index) stay. The top_k best
  * experts' indices go to ids [tokens, top_k], best first, their s (without the
  * bias) to weights, divided by their sum if renormalise, times scale.
- * A sigmoid logit under -87 scores 0. A logit of -inf or NaN (or such a
- * bias) takes its expert out; where fewer
- * than top_k experts are left, the rest of ids is -1 with weight 0, and so is
- * every entry of a token whose mask byte is 0 (mask [tokens] or NULL).
+ * A sigmoid logit under -87 scores 0. A logit of -inf or NaN (or such a bias)
+ * takes its expert out; where fewer than top_k experts are left, the rest of
+ * ids is -1 with weight 0, and so is every entry of a token whose mask byte is
+ * 0 (mask [tokens] or NULL).
  * top_k must not exceed the experts of groups_kept groups. */
 typedef enum tpt_score { TPT_SCORE_SOFTMAX = 0, TPT_SCORE_SIGMOID = 1 } tpt_score;
 #define TPT_ROUTE_MAX_EXPERTS 1024
@@ -457,7 +459,7 @@ int tpt_cuda_route_experts_dev(tpt_cuda_ctx *ctx, const void *logits, int dtype,
  * tpt_cuda_route_experts_dev writes them (a negative id is no expert; an id
  * past the last expert counts as none and makes the next synchronising call
  * return TPT_DEVICE_CHECK). h is rounded to the operands' type between the
- * two products; the sum over j is in f32, in the order of j. */
+ * two products; the sum over j is in f32, in a fixed order. */
 #define TPT_EXPERTS_MAX 4096
 int tpt_cuda_experts_mlp_dev(tpt_cuda_ctx *ctx, int dtype, const void *x, size_t ldx, size_t tokens, size_t d,
                              const int32_t *ids, const float *weights, size_t top_k, const void *w_in,

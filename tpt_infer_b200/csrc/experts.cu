@@ -611,7 +611,7 @@ int tpt_cuda_route_experts_dev(tpt_cuda_ctx *ctx, const void *logits, int dtype,
     if (dtype != TPT_DT_F32 && dtype != TPT_DT_BF16 && dtype != TPT_DT_F16) return TPT_UNSUPPORTED;
     if (score != TPT_SCORE_SOFTMAX && score != TPT_SCORE_SIGMOID) return TPT_INVALID;
     if (experts == 0 || top_k == 0 || groups == 0 || groups_kept == 0) return TPT_INVALID;
-    if (experts > TPT_ROUTE_MAX_EXPERTS || top_k > TPT_ROUTE_MAX_TOP_K || groups > 32 || tokens > 0x7fffffff)
+    if (experts > TPT_ROUTE_MAX_EXPERTS || top_k > TPT_ROUTE_MAX_TOP_K || groups > 32 || tokens > TPT_LINEAR_MAX)
         return TPT_UNSUPPORTED;
     if (experts % groups || groups_kept > groups || (group_top != 1 && group_top != 2)) return TPT_INVALID;
     if (top_k > groups_kept * (experts / groups)) return TPT_INVALID;
@@ -643,7 +643,7 @@ int tpt_cuda_experts_mlp_dev(tpt_cuda_ctx *ctx, int dtype, const void *x, size_t
     cudaSetDevice(ctx->device);
     if (dtype != TPT_DT_BF16 && dtype != TPT_DT_F16) return TPT_UNSUPPORTED;
     if (act < 0 || act > TPT_ACT_SILU || experts == 0 || top_k == 0 || f == 0) return TPT_INVALID;
-    if (tokens > 0x7fffffff || d > 0x3fffffff || f > 0x3fffffff || experts > TPT_EXPERTS_MAX ||
+    if (tokens > TPT_LINEAR_MAX || d > TPT_LINEAR_MAX || f > TPT_LINEAR_MAX || experts > TPT_EXPERTS_MAX ||
         top_k > TPT_EXPERTS_MAX)
         return TPT_UNSUPPORTED;
     if (tokens == 0 || d == 0) return TPT_OK;

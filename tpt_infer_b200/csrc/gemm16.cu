@@ -127,7 +127,7 @@ int tpt_cuda_linear_dev(tpt_cuda_ctx *ctx, int dtype, const void *x, size_t ldx,
     if (dtype != TPT_DT_BF16 && dtype != TPT_DT_F16) return TPT_UNSUPPORTED;
     if (y_dtype != dtype && y_dtype != TPT_DT_F32) return TPT_UNSUPPORTED;
     if (act < 0 || act > TPT_ACT_SILU) return TPT_INVALID;
-    if (m > 0x7fffffff || n > 0x7fffffff || k > 0x7fffffff) return TPT_UNSUPPORTED;
+    if (m > TPT_LINEAR_MAX || n > TPT_LINEAR_MAX || k > TPT_LINEAR_MAX) return TPT_UNSUPPORTED;
     if (m == 0 || n == 0) return TPT_OK;
     if (!y || (k && (!x || !w))) return TPT_INVALID;
     if ((m > 1 && (ldx < k || ldy < n || (residual && ldr < n))) || (n > 1 && ldw < k)) return TPT_SHAPE_MISMATCH;

@@ -384,7 +384,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                     stage = S - 1;
                     phase ^= 1u;
                 }
-                warp_wait(full_bar(stage), phase, abort_p, a.gflags, false);
+                // (it gives up with the first that never fills: the other CTA stopped too)
+                if (!warp_wait(full_bar(stage), phase, abort_p, a.gflags, false)) break;
             }
         }
     } else if (warp == 1) {
@@ -548,6 +549,11 @@ __global__ void __launch_bounds__(S_THREADS, 2)
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmW)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
     }
+    // Tensor memory is taken after the wait: a CTA of the kernel before that has yet
+    // to allocate its own may share this SM, and would wait for this one while this
+    // one waited for it. And before the trigger, for the kernel after in turn. (The
+    // pair kernel's shared memory leaves no room for such a neighbour.)
+    pdl_wait();
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
                      "r"((uint32_t)Cfg::TMEM_COLS)
@@ -557,7 +563,6 @@ __global__ void __launch_bounds__(S_THREADS, 2)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    pdl_wait();
     pdl_trigger();
     const uint32_t tmem = tmem_slot;
     volatile int *abort_p = &abort_flag;
