@@ -26,15 +26,17 @@ __device__ __forceinline__ void pad_row(uintptr_t first, uintptr_t last, uintptr
                 w[j / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(at + 2 * j)) << (16 * (j & 1));
         return make_uint4(w[0], w[1], w[2], w[3]);
     };
-    for (size_t p0 = 0; p0 < pieces; p0 += 124) {  // 31 pieces a load: the last lane's word is its neighbour's next
-        uint4 v[4];
+    constexpr int U = 6;  // loads in flight
+    for (size_t p0 = 0; p0 < pieces; p0 += 31 * U) {  // 31 pieces a load: the last lane's word is its neighbour's next
+        uint4 v[U];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < U; u++) {
             const size_t c = p0 + 31 * u + lane;
             v[u] = c <= pieces ? word(c) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < U; u++) {
+            if (p0 + 31 * u >= pieces) break;
             const size_t c = p0 + 31 * u + lane;
             uint32_t w[8] = {v[u].x, v[u].y, v[u].z, v[u].w,
                              __shfl_down_sync(0xffffffffu, v[u].x, 1), __shfl_down_sync(0xffffffffu, v[u].y, 1),
