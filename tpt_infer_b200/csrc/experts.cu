@@ -446,7 +446,7 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
     // 2048 x 768, 8 chosen: 1 token 24 us against 29, 4 tokens 57 against 58; 8 tokens of
     // 64 experts, 4 chosen: 30 against 24).
     const bool stream = tokens <= 4 && tokens * top_k <= STREAM_PAIRS && stream_x_bytes(tokens, d) <= STREAM_X_BYTES &&
-                        stream_x_bytes(tokens * top_k, f) <= STREAM_X_BYTES;
+                        stream_x_bytes(2 * tokens * top_k, f) <= STREAM_X_BYTES;
     // With tiles of 16 tokens the product gathers x's rows itself (TMA, four rows
     // an instruction, ~20 cycles a row): no launch and no copy. Longer tiles would
     // wait for those rows (8192 tokens: 1192 us gathered, 49 + 355 us spread), and x is

@@ -51,15 +51,16 @@ struct Gemm16 {
 int launch_gemm16(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g);
 
 // The kernels of a few tokens, for operands like launch_gemm16's: a dense product of
-// up to STREAM_TOKENS rows, and both of the experts' products of up to
-// STREAM_PAIRS (token, choice) pairs of up to 8 tokens. `in` reads the tokens'
-// rows and writes [tile][8][ldy], one tile per distinct expert; `out` reads
-// those and writes the tokens' weighted sums.
-// The tokens' rows have to fit STREAM_X_BYTES of shared memory.
-// (4 x 4096 x 4096: 8.5 us against the split kernel's 10; 8 x 4096 x 11008: 21.3
-// against 18.2, since every block holds every token's row.)
+// up to STREAM_TOKENS rows, and both of the experts' products of as many tokens and
+// up to STREAM_PAIRS (token, choice) pairs. `in` reads the tokens' rows and writes
+// [tile][4][2][ldy], one tile per distinct expert; `out` reads those and writes the
+// tokens' weighted sums. (4 x 4096 x 4096: 8.5 us against the split kernel's 10; 8 x 4096
+// x 11008: 21.3 against 18.2, since every block reads and holds every token's row.)
+// Those rows have to fit STREAM_X_BYTES of shared memory: it is taken from the L1
+// that the weights in flight need (with the largest carveout 1 x 4096 x 4096 takes 11 us
+// instead of 7).
 constexpr int STREAM_TOKENS = 4, STREAM_PAIRS = 32;
-constexpr size_t STREAM_X_BYTES = 80 * 1024;
+constexpr size_t STREAM_X_BYTES = 52 * 1024;
 inline size_t stream_x_bytes(size_t rows, size_t k) { return rows * ((k + 63) / 64 * 128 + 16); }
 int launch_gemm16_stream(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g);
 int launch_experts_stream(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &in, const Gemm16 &out, const int *ids,

@@ -69,8 +69,12 @@ __device__ __forceinline__ uint4 load8(const uint16_t *p, bool in) {
 }
 
 // GATED: y = act(W x) * (W2 x). SUM: y[token] = sum over the experts of
-// weight * W_e x_e, x the tiles' rows [tile][token]; otherwise each tile's
-// products go to y's rows [tile][token] (dense: one tile). Up to 8 tokens.
+// weight * W_e h_e, h the tiles' rows [tile][token]; otherwise a tile's products go
+// to h's rows [tile][token] (dense: to y). Up to 4 tokens. A row of h is two rows of
+// 16-bit values, the products rounded and what that rounding left, and they take two
+// of the MMA's 8 columns: a token's result comes from a few thousand values of h, and
+// how the largest of them happen to round would show in it (up to 1.55 times the
+// error of one rounded y).
 template <typename T, typename TY, bool GATED, bool SUM>
 __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant__ StreamArgs a) {
     constexpr int H = GATED ? 2 : 1;
@@ -79,9 +83,9 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
     __shared__ float red[2][ST_WARPS][H][ST_ROWS][COLS];
     __shared__ int tile_expert[32];
     // SUM: per tile the tokens that chose the expert, per tile and token its weight
-    // and its staged row, per staged row its tile * 8 + token
-    __shared__ int tile_used[SUM ? 32 : 1], slot_of[SUM ? 256 : 1], slot_row[SUM ? 32 : 1];
-    __shared__ float tile_w[SUM ? 256 : 1];
+    // and its staged row, per staged row its tile * 4 + token
+    __shared__ int tile_used[SUM ? 32 : 1], slot_of[SUM ? 128 : 1], slot_row[SUM ? 32 : 1];
+    __shared__ float tile_w[SUM ? 128 : 1];
     extern __shared__ __align__(16) uint8_t xs[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -127,7 +131,7 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
         if (warp == 0 && valid && leader == lane) tile_expert[tile] = id;
         if (SUM) {
             // a token that chose the expert twice takes it once, with both weights
-            const unsigned twin = __match_any_sync(0xffffffffu, valid ? id * 8 + tok : -1 - lane);
+            const unsigned twin = __match_any_sync(0xffffffffu, valid ? id * 4 + tok : -1 - lane);
             const bool row = valid && __ffs(twin) - 1 == lane;
             const unsigned slots = __ballot_sync(0xffffffffu, row);
             x_rows = __popc(slots);
@@ -141,9 +145,9 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
             }
             if (warp == 0 && row) {
                 const int slot = __popc(slots & below);
-                slot_row[slot] = tile * 8 + tok;
-                slot_of[tile * 8 + tok] = slot;
-                tile_w[tile * 8 + tok] = sum;
+                slot_row[slot] = tile * 4 + tok;
+                slot_of[tile * 4 + tok] = slot;
+                tile_w[tile * 4 + tok] = sum;
             }
             if (warp == 0 && valid && leader == lane) {
                 int used = 0;
@@ -230,10 +234,12 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
     // to the next, so that eight rows' fragments lie in different banks
     const int xld = kch * ST_CHUNK * 2 + 16;
     const int pieces = kch * (ST_CHUNK / 8);  // of 16 bytes, a row
-    for (int i = threadIdx.x; i < x_rows * pieces; i += ST_T) {  // all in flight together
+    // (SUM: the upper halves of h's rows, then the lower ones)
+    for (int i = threadIdx.x; i < (SUM ? 2 : 1) * x_rows * pieces; i += ST_T) {  // all in flight together
         const int r = i / pieces, c = (i - r * pieces) * 8;
         const int n = min(max(a.k - c, 0), 8);  // values of this piece
-        const uint16_t *src = x + (size_t)(SUM ? slot_row[r] : r) * a.ldx;
+        const int low = SUM && r >= x_rows ? 1 : 0;
+        const uint16_t *src = x + (size_t)(SUM ? slot_row[r - low * x_rows] * 2 + low : r) * a.ldx;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(xs) + r * xld + c * 2),
                      "l"(src + (n ? c : 0)), "r"(n * 2)
                      : "memory");
@@ -253,10 +259,12 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
         float acc[H][4] = {}, sum[4] = {};
         bool more = kc < last;
         while (more) {
-            // this lane's column is token g
+            // this lane's column: token g, or, summing, token g % 4 and the upper (g < 4)
+            // or lower half of its row
             const int used = SUM ? tile_used[tile] : 0;
-            const bool in = SUM ? (used >> g & 1) != 0 : g < a.tokens;
-            const uint8_t *xp = xs + (in && SUM ? slot_of[tile * 8 + g] : g) * xld + 16 * t;
+            const bool in = SUM ? (used >> (g & 3) & 1) != 0 : g < a.tokens;
+            const int xrow = SUM ? (in ? slot_of[tile * 4 + (g & 3)] + (g >> 2) * x_rows : 0) : g;
+            const uint8_t *xp = xs + xrow * xld + 16 * t;
             wait_staged();
 #pragma unroll
             for (int d = 0; d < DEPTH; d++) {
@@ -289,9 +297,9 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
             if (SUM && seg_end) {  // the warp's share of this expert's products: weigh it
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int tok = 2 * t + (i & 1);
+                    const int tok = (2 * t + (i & 1)) & 3;
                     // a token without this expert takes nothing of it, not 0 x inf
-                    if (used >> tok & 1) sum[i] = fmaf(tile_w[weigh * 8 + tok], acc[0][i], sum[i]);
+                    if (used >> tok & 1) sum[i] = fmaf(tile_w[weigh * 4 + tok], acc[0][i], sum[i]);
                     acc[0][i] = 0.0f;
                 }
             }
@@ -315,14 +323,22 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
 #pragma unroll
             for (int i = 0; i < ST_WARPS; i++) {
                 v[0] += red[rb][i][0][r][o];
+                if (SUM) v[0] += red[rb][i][0][r][o + 4];
                 if (GATED) u += red[rb][i][H - 1][r][o];
             }
             if (a.bias) v[0] += to_f32(static_cast<const T *>(a.bias)[g_f + r]);
             act16(v, a.act);
             if (GATED) v[0] *= u;
             if (a.residual) v[0] += to_f32(static_cast<const TY *>(a.residual)[(size_t)o * a.ldr + g_f + r]);
-            const size_t row = a.ids && !SUM ? (size_t)g_tile * 8 + o : (size_t)o;
-            static_cast<TY *>(a.y)[row * a.ldy + g_f + r] = from_f32<TY>(v[0]);
+            if (a.ids && !SUM) {
+                TY *h = static_cast<TY *>(a.y) + ((size_t)g_tile * 4 + o) * 2 * a.ldy + g_f + r;
+                const TY upper = from_f32<TY>(v[0]);
+                const float rest = v[0] - to_f32(upper);
+                h[0] = upper;
+                h[a.ldy] = from_f32<TY>(isfinite(rest) ? rest : 0.0f);  // inf - inf stays out
+            } else {
+                static_cast<TY *>(a.y)[(size_t)o * a.ldy + g_f + r] = from_f32<TY>(v[0]);
+            }
         }
         rb ^= 1;  // the next group's sums go beside these; the barrier after it frees them
     }
@@ -382,7 +398,7 @@ int experts_typed(tpt_cuda_ctx *ctx, const Gemm16 &in, const Gemm16 &out, const 
     const long long rows = (long long)in.n * (pairs < in.experts ? pairs : in.experts);
     const int st = in.gated ? launch<T, T, true, false>(ctx, a, rows, a.tokens)
                             : launch<T, T, false, false>(ctx, a, rows, a.tokens);
-    return st ? st : launch<T, T, false, true>(ctx, b, out.n, pairs);
+    return st ? st : launch<T, T, false, true>(ctx, b, out.n, 2 * pairs);
 }
 
 }  // namespace
