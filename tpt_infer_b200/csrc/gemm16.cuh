@@ -44,6 +44,11 @@ struct Gemm16 {
     void *y = nullptr;
     size_t ldy = 0;
     bool y_f32 = false;
+    // Two planes of 16-bit values for 16 bits of the numbers between two products:
+    // y's second plane (y_low elements on) takes what y's rounding left, X's second
+    // plane (x_low rows on) is added to the first. X's only with tiles of 16 rows, f32 y.
+    size_t y_low = 0;
+    int x_low = 0;
 };
 
 // Device enqueue; dtype TPT_DT_BF16 or TPT_DT_F16, k > 0. The operands' rows

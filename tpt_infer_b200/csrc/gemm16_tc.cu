@@ -48,6 +48,8 @@ struct Args {
     size_t ldr;
     void *y;
     size_t ldy;
+    size_t low;                  // y's second plane (elements on) takes what y's rounding left; 0: none
+    int x_low;                   // X's second plane (rows on), added to the first in the products
     unsigned *gflags;
 };
 
@@ -170,6 +172,17 @@ __device__ __forceinline__ void load_residual(const Args &a, TY (&rv)[C], int f,
     }
 }
 
+// One output, and with `low` what its rounding left, for a product that reads both
+template <typename TY>
+__device__ __forceinline__ void store16(TY *y, float v, size_t low) {
+    const TY upper = from_f32<TY>(v);
+    *y = upper;
+    if (low) {
+        const float rest = v - to_f32(upper);
+        y[low] = from_f32<TY>(isfinite(rest) ? rest : 0.0f);  // inf - inf stays out
+    }
+}
+
 // The epilogue of C columns of this thread's lane. Ungated: lane l of the warp
 // is feature f0 + l, b its bias, rv its residual values.
 template <typename TY, int C>
@@ -186,11 +199,11 @@ __device__ __forceinline__ void epilogue16(const Args &a, float (&v)[C], const T
     TY *y = static_cast<TY *>(a.y) + (row0 + col0) * a.ldy + f;
     if (n >= C) {
 #pragma unroll
-        for (int i = 0; i < C; i++, y += a.ldy) *y = from_f32<TY>(v[i]);
+        for (int i = 0; i < C; i++, y += a.ldy) store16(y, v[i], a.low);
     } else {
 #pragma unroll
         for (int i = 0; i < C; i++, y += a.ldy)
-            if (i < n) *y = from_f32<TY>(v[i]);
+            if (i < n) store16(y, v[i], a.low);
     }
 }
 // Gated: lanes l and l + 16 are the gate and the up product of feature f0 + l;
@@ -213,11 +226,11 @@ __device__ __forceinline__ void epilogue16_gated(const Args &a, const float (&v)
     const int n = f < a.n ? rows - c0 : 0;
     if (n >= C / 2) {
 #pragma unroll
-        for (int i = 0; i < C / 2; i++, y += a.ldy) *y = from_f32<TY>(g[i] * u[i]);
+        for (int i = 0; i < C / 2; i++, y += a.ldy) store16(y, g[i] * u[i], a.low);
     } else {
 #pragma unroll
         for (int i = 0; i < C / 2; i++, y += a.ldy)
-            if (i < n) *y = from_f32<TY>(g[i] * u[i]);
+            if (i < n) store16(y, g[i] * u[i], a.low);
     }
 }
 // the bias of feature f (0: none)
@@ -510,22 +523,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
 // ---------------------------------------------------------------------------
 constexpr int S_THREADS = 6 * 32;
 
-template <int NT>
+// LOW: X has two planes, the tokens' values and what their rounding left; the second
+// one's rows are further columns, added to the first's.
+template <int NT, bool LOW>
 struct SplitCfg {
-    static constexpr int STAGE_BYTES = W_BYTES + NT * ROW_BYTES;
-    static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 3;
-    static constexpr int TMEM_COLS = NT < 32 ? 32 : NT;
+    static constexpr int COLS = LOW ? 2 * NT : NT;  // the MMA's
+    static constexpr int STAGE_BYTES = W_BYTES + COLS * ROW_BYTES;
+    static constexpr int STAGES = COLS == 16 ? 6 : COLS == 32 ? 5 : COLS == 64 ? 4 : 3;
+    static constexpr int TMEM_COLS = COLS < 32 ? 32 : COLS;
     static constexpr int SMEM = STAGES * STAGE_BYTES + (2 * STAGES + 1) * 8 + 1024;
-
     static_assert(2 * (SMEM + 1024) <= 233472, "two CTAs per SM");
 };
 
-template <typename T, typename TY, bool GATED, int NT, int KS>
+// 16 columns of this thread's lane, with LOW the second plane's added
+template <bool LOW>
+__device__ __forceinline__ void load16(uint32_t taddr, float (&v)[16]) {
+    float w[16];
+    tmem_ld16(taddr, reinterpret_cast<uint32_t *>(v));
+    if (LOW) tmem_ld16(taddr + 16, reinterpret_cast<uint32_t *>(w));
+    tmem_wait_ld();
+    if (LOW) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] += w[i];
+    }
+}
+
+template <typename T, typename TY, bool GATED, int NT, int KS, bool LOW>
 __global__ void __launch_bounds__(S_THREADS, 2)
     k_gemm16_split(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                    const __grid_constant__ Args a) {
-    using Cfg = SplitCfg<NT>;
+    using Cfg = SplitCfg<NT, LOW>;
     constexpr int S = Cfg::STAGES;
+    static_assert(!LOW || NT == 16, "the epilogue adds columns i and i + 16");
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag;
     __shared__ uint32_t tmem_slot;
@@ -613,6 +642,7 @@ __global__ void __launch_bounds__(S_THREADS, 2)
                         tma_load_3d(w_dst, &tmW, fb, kb * BK, ft * 128, expert);
                     }
                     if (!a.row_token) tma_load_2d(x_dst, &tmX, fb, kb * BK, row0);
+                    if (LOW) tma_load_2d(x_dst + NT * ROW_BYTES, &tmX, fb, kb * BK, row0 + a.x_low);
                 }
                 __syncwarp();
                 if (a.row_token && lane * 4 < NT) tma_gather4(x_dst + lane * 4 * ROW_BYTES, &tmX, fb, kb * BK, r4);
@@ -634,7 +664,7 @@ __global__ void __launch_bounds__(S_THREADS, 2)
             }
         } else if (warp == 1) {
             // ---------------- MMA issuer ----------------
-            const uint32_t idesc = idesc_f16(a.fmt, 128, NT);
+            const uint32_t idesc = idesc_f16(a.fmt, 128, Cfg::COLS);
             int stage = 0;
             uint32_t phase = 0;
             for (int kb = kb0; kb < kb1; kb++) {
@@ -679,11 +709,12 @@ __global__ void __launch_bounds__(S_THREADS, 2)
                     if (!GATED && a.residual) load_residual<TY, C>(a, rv, f0 + lane, (size_t)row0, c, rows);
                     float v[C];
                     __syncwarp();
-                    if constexpr (C == 32)
+                    if constexpr (C == 32) {
                         tmem_ld32(t_base + (uint32_t)c, reinterpret_cast<uint32_t(&)[32]>(v));
-                    else
-                        tmem_ld16(t_base + (uint32_t)c, reinterpret_cast<uint32_t *>(v));
-                    tmem_wait_ld();
+                        tmem_wait_ld();
+                    } else {
+                        load16<LOW>(t_base + (uint32_t)c, v);
+                    }
                     if constexpr (GATED)
                         epilogue16_gated<TY, C>(a, v, f0, (size_t)row0, c, rows, lane);
                     else
@@ -700,15 +731,14 @@ __global__ void __launch_bounds__(S_THREADS, 2)
             if (warp >= 2) {
 #pragma unroll 1
                 for (int c = 0; c < NT && c < rows; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld16(t_base + (uint32_t)c, v);
-                    tmem_wait_ld();
+                    float v[16];
+                    load16<LOW>(t_base + (uint32_t)c, v);
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
                         const int o = (c + i) / CW, oc = (c + i) % CW;
                         const uint32_t dst = map_to_rank(ring, (uint32_t)o) +
                                              (uint32_t)(((rank * CW + oc) * W_ROWS + q * 32 + lane) * 4);
-                        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(dst), "r"(v[i]) : "memory");
+                        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(dst), "f"(v[i]) : "memory");
                     }
                 }
             }
@@ -817,6 +847,8 @@ Args make_args(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
     a.ldr = g.ldr;
     a.y = g.y;
     a.ldy = g.ldy;
+    a.low = g.y_low;
+    a.x_low = g.x_low;
     a.gflags = ctx->d_flags;
     return a;
 }
@@ -890,10 +922,10 @@ int pair_tile_n(tpt_cuda_ctx *ctx, const Gemm16 &g) {
     return best_n;
 }
 
-template <typename T, typename TY, bool GATED, int NT, int KS>
+template <typename T, typename TY, bool GATED, int NT, int KS, bool LOW>
 int launch_split(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
-    using Cfg = SplitCfg<NT>;
-    auto kern = k_gemm16_split<T, TY, GATED, NT, KS>;
+    using Cfg = SplitCfg<NT, LOW>;
+    auto kern = k_gemm16_split<T, TY, GATED, NT, KS, LOW>;
     static bool done[64] = {};
     const int dev = ctx->device & 63;
     if (!done[dev]) {
@@ -929,15 +961,15 @@ int launch_split(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
     return after_launch(ctx, "gemm16_split");
 }
 
-template <typename T, typename TY, bool GATED, int NT>
+template <typename T, typename TY, bool GATED, int NT, bool LOW = false>
 int launch_split_k(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g, int ks) {
     switch (ks) {
-        case 8: return launch_split<T, TY, GATED, NT, 8>(ctx, dtype, g);
-        case 6: return launch_split<T, TY, GATED, NT, 6>(ctx, dtype, g);
-        case 4: return launch_split<T, TY, GATED, NT, 4>(ctx, dtype, g);
-        case 3: return launch_split<T, TY, GATED, NT, 3>(ctx, dtype, g);
-        case 2: return launch_split<T, TY, GATED, NT, 2>(ctx, dtype, g);
-        default: return launch_split<T, TY, GATED, NT, 1>(ctx, dtype, g);
+        case 8: return launch_split<T, TY, GATED, NT, 8, LOW>(ctx, dtype, g);
+        case 6: return launch_split<T, TY, GATED, NT, 6, LOW>(ctx, dtype, g);
+        case 4: return launch_split<T, TY, GATED, NT, 4, LOW>(ctx, dtype, g);
+        case 3: return launch_split<T, TY, GATED, NT, 3, LOW>(ctx, dtype, g);
+        case 2: return launch_split<T, TY, GATED, NT, 2, LOW>(ctx, dtype, g);
+        default: return launch_split<T, TY, GATED, NT, 1, LOW>(ctx, dtype, g);
     }
 }
 
@@ -962,6 +994,8 @@ int launch_tc(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
     int ks = 1;
     for (int s : {2, 3, 4, 6, 8})
         if (tiles * s <= 2LL * ctx->sm_count && kb / s >= 3 && (nt < 128 || s <= 4)) ks = s;
+    if constexpr (!GATED && std::is_same<TY, float>::value)
+        if (g.x_low) return launch_split_k<T, TY, GATED, 16, true>(ctx, dtype, g, ks);  // tiles of 16: the caller's choice
     if (nt == 16) return launch_split_k<T, TY, GATED, 16>(ctx, dtype, g, ks);
     if (nt == 32) return launch_split_k<T, TY, GATED, 32>(ctx, dtype, g, ks);
     if (nt == 64) return launch_split_k<T, TY, GATED, 64>(ctx, dtype, g, ks);
