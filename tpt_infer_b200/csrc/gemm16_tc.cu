@@ -173,11 +173,13 @@ __device__ __forceinline__ void load_residual(const Args &a, TY (&rv)[C], int f,
 }
 
 // One output, and with `low` what its rounding left, for a product that reads both
-template <typename TY>
+// (a template argument too: the test alone makes the pair kernel's epilogue a
+// quarter longer)
+template <bool LOW, typename TY>
 __device__ __forceinline__ void store16(TY *y, float v, size_t low) {
     const TY upper = from_f32<TY>(v);
     *y = upper;
-    if (low) {
+    if (LOW && low) {
         const float rest = v - to_f32(upper);
         y[low] = from_f32<TY>(isfinite(rest) ? rest : 0.0f);  // inf - inf stays out
     }
@@ -185,7 +187,7 @@ __device__ __forceinline__ void store16(TY *y, float v, size_t low) {
 
 // The epilogue of C columns of this thread's lane. Ungated: lane l of the warp
 // is feature f0 + l, b its bias, rv its residual values.
-template <typename TY, int C>
+template <bool LOW, typename TY, int C>
 __device__ __forceinline__ void epilogue16(const Args &a, float (&v)[C], const TY (&rv)[C], float b, int f, size_t row0,
                                            int col0, int rows) {
     const int n = f < a.n ? rows - col0 : 0;
@@ -199,16 +201,16 @@ __device__ __forceinline__ void epilogue16(const Args &a, float (&v)[C], const T
     TY *y = static_cast<TY *>(a.y) + (row0 + col0) * a.ldy + f;
     if (n >= C) {
 #pragma unroll
-        for (int i = 0; i < C; i++, y += a.ldy) store16(y, v[i], a.low);
+        for (int i = 0; i < C; i++, y += a.ldy) store16<LOW>(y, v[i], a.low);
     } else {
 #pragma unroll
         for (int i = 0; i < C; i++, y += a.ldy)
-            if (i < n) store16(y, v[i], a.low);
+            if (i < n) store16<LOW>(y, v[i], a.low);
     }
 }
 // Gated: lanes l and l + 16 are the gate and the up product of feature f0 + l;
 // each of them finishes half of the columns.
-template <typename TY, int C>
+template <bool LOW, typename TY, int C>
 __device__ __forceinline__ void epilogue16_gated(const Args &a, const float (&v)[C], int f0, size_t row0, int col0,
                                                  int rows, int lane) {
     const bool hi = lane >= 16;
@@ -226,11 +228,11 @@ __device__ __forceinline__ void epilogue16_gated(const Args &a, const float (&v)
     const int n = f < a.n ? rows - c0 : 0;
     if (n >= C / 2) {
 #pragma unroll
-        for (int i = 0; i < C / 2; i++, y += a.ldy) store16(y, g[i] * u[i], a.low);
+        for (int i = 0; i < C / 2; i++, y += a.ldy) store16<LOW>(y, g[i] * u[i], a.low);
     } else {
 #pragma unroll
         for (int i = 0; i < C / 2; i++, y += a.ldy)
-            if (i < n) store16(y, g[i] * u[i], a.low);
+            if (i < n) store16<LOW>(y, g[i] * u[i], a.low);
     }
 }
 // the bias of feature f (0: none)
@@ -490,9 +492,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                 tmem_ld32(t_base + (uint32_t)c, reinterpret_cast<uint32_t(&)[32]>(v));
                 tmem_wait_ld();
                 if constexpr (GATED)
-                    epilogue16_gated<TY, 32>(a, v, f0, (size_t)tl.row0, c, tl.rows, lane);
+                    epilogue16_gated<false, TY, 32>(a, v, f0, (size_t)tl.row0, c, tl.rows, lane);
                 else
-                    epilogue16<TY, 32>(a, v, rv[i & 1], b, f0 + lane, (size_t)tl.row0, c, tl.rows);
+                    epilogue16<false, TY, 32>(a, v, rv[i & 1], b, f0 + lane, (size_t)tl.row0, c, tl.rows);
             }
             tc_fence_before();
             __syncwarp();
@@ -554,6 +556,7 @@ __global__ void __launch_bounds__(S_THREADS, 2)
                    const __grid_constant__ Args a) {
     using Cfg = SplitCfg<NT, LOW>;
     constexpr int S = Cfg::STAGES;
+    constexpr bool LOW_OUT = NT == 16 && std::is_same<T, TY>::value;  // may write a second plane
     static_assert(!LOW || NT == 16, "the epilogue adds columns i and i + 16");
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag;
@@ -716,9 +719,9 @@ __global__ void __launch_bounds__(S_THREADS, 2)
                         load16<LOW>(t_base + (uint32_t)c, v);
                     }
                     if constexpr (GATED)
-                        epilogue16_gated<TY, C>(a, v, f0, (size_t)row0, c, rows, lane);
+                        epilogue16_gated<LOW_OUT, TY, C>(a, v, f0, (size_t)row0, c, rows, lane);
                     else
-                        epilogue16<TY, C>(a, v, rv, b, f0 + lane, (size_t)row0, c, rows);
+                        epilogue16<LOW_OUT, TY, C>(a, v, rv, b, f0 + lane, (size_t)row0, c, rows);
                 }
             }
         } else {
@@ -759,9 +762,9 @@ __global__ void __launch_bounds__(S_THREADS, 2)
                         for (int s = 1; s < KS; s++) v[i] += part[(s * CW + c - c0 + i) * W_ROWS];
                     }
                     if constexpr (GATED)
-                        epilogue16_gated<TY, C>(a, v, f0, (size_t)row0, c, rows, lane);
+                        epilogue16_gated<LOW_OUT, TY, C>(a, v, f0, (size_t)row0, c, rows, lane);
                     else
-                        epilogue16<TY, C>(a, v, rv, b, f0 + lane, (size_t)row0, c, rows);
+                        epilogue16<LOW_OUT, TY, C>(a, v, rv, b, f0 + lane, (size_t)row0, c, rows);
                     __syncwarp();
                 }
             }
