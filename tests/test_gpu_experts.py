@@ -350,6 +350,30 @@ def test_experts_bad_weights_stay_in_their_features(cuda, bad, t):
         assert not torch.isfinite(y[hit, 70]).any()
 
 
+@pytest.mark.parametrize("ty", ["bf16", "f16"])
+@pytest.mark.parametrize("t", [1, 4, 12, 60])
+def test_experts_infinite_weight_gives_infinity(cuda, t, ty):
+    """An infinite weight of one output makes it +inf or -inf, as the hidden value's sign says, not NaN: also where
+    the hidden values are kept in two parts, whose signs differ."""
+    import torch
+
+    x, ids, wts, w_in, w_out = expert_inputs(t, 3, 2, 200, 72, ty, True)
+    ids[:, 1] = -1  # one expert a token
+    y = torch.empty_like(x)
+    torch.cuda.synchronize()
+    for k in range(72):  # every hidden value in turn, so that both signs of both parts come up
+        w_out[:, 70, :] = 0
+        w_out[:, 70, k] = float("inf")
+        torch.cuda.synchronize()
+        cuda.experts_mlp_dev(x, ids, wts, w_in, w_out, 3, True, None, y)
+        cuda.sync()
+        wi = w_in.double()[ids[:, 0].long()]
+        gate, up = (wi[:, k] * x.double()).sum(1), (wi[:, 72 + k] * x.double()).sum(1)
+        h = act64(gate, "silu") * up
+        sure = h.abs() > 1e-3  # the products' errors are under 1e-4, and f16 holds it
+        assert torch.equal(y[sure, 70].double(), h[sure].sign() * float("inf"))
+
+
 def test_experts_many_tokens_in_chunks(cuda):
     """More intermediate results than the workspace takes at once."""
     x, ids, wts, w_in, w_out = expert_inputs(17000, 8, 8, 4096, 64, "bf16", True)

@@ -120,6 +120,10 @@ __device__ __forceinline__ __half from_f32<__half>(float v) {
     return __float2half_rn(v);
 }
 
+// A sum over the values' upper parts and the one over their lower parts. An infinite
+// weight makes the first what it is and the second an infinity of any sign, or 0 x inf.
+__device__ __forceinline__ float add_low(float upper, float lower) { return isfinite(upper) ? upper + lower : upper; }
+
 // The activations of the 16-bit products' epilogues, C values in place; act is
 // uniform, so the choice is one branch for all of them. Both smooth ones are
 // x / (1 + e^-z) with the hardware's exponential and quotient (errors of a few

@@ -319,13 +319,14 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
         // one output a thread: feature g_f + r of token o
         const int r = threadIdx.x & 15, o = threadIdx.x >> 4;
         if (o < COLS && o < a.tokens && r < g_rows) {
-            float v[1] = {0.0f}, u = 0.0f;
+            float v[1] = {0.0f}, u = 0.0f, rest = 0.0f;
 #pragma unroll
             for (int i = 0; i < ST_WARPS; i++) {
                 v[0] += red[rb][i][0][r][o];
-                if (SUM) v[0] += red[rb][i][0][r][o + 4];
+                if (SUM) rest += red[rb][i][0][r][o + 4];
                 if (GATED) u += red[rb][i][H - 1][r][o];
             }
+            if (SUM) v[0] = add_low(v[0], rest);
             if (a.bias) v[0] += to_f32(static_cast<const T *>(a.bias)[g_f + r]);
             act16(v, a.act);
             if (GATED) v[0] *= u;

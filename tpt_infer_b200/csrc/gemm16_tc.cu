@@ -546,7 +546,7 @@ __device__ __forceinline__ void load16(uint32_t taddr, float (&v)[16]) {
     tmem_wait_ld();
     if (LOW) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) v[i] += w[i];
+        for (int i = 0; i < 16; i++) v[i] = add_low(v[i], w[i]);
     }
 }
 
