@@ -269,3 +269,33 @@ def test_refusals(cuda):
     assert lib.tpt_cuda_linear_dev(cuda.ctx, 7, p(x), 8, 2, 8, p(w), 8, 4, None, 0, None, 0, p(y), 4, 7) == 3
     assert lib.tpt_cuda_linear_dev(cuda.ctx, bf, p(x), 8, 1 << 31, 8, p(w), 8, 4, None, 0, None, 0, p(y), 4, bf) == 3
     cuda.sync()
+
+
+@pytest.mark.parametrize("m,k,n", [(16, 4096, 32768), (48, 4096, 2048)])  # whole k in a CTA; k split over a cluster
+def test_linear_wait_limit_reports_a_timeout_and_the_context_recovers(cuda, m, k, n):
+    """With the wait limit cut to 100 cycles the waits of a normal launch run out over its loads from memory: the
+    kernel leaves, the host reads a timeout, and with the default limit the next call is right."""
+    import torch
+
+    from tpt_infer_b200 import OpError
+    from tpt_infer_b200._capi import lib
+
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x = torch.randn(m, k, generator=g, device="cuda").bfloat16()
+    w = torch.randn(n, k, generator=g, device="cuda").bfloat16()
+    y = torch.empty(m, n, device="cuda")
+    torch.cuda.synchronize()
+    try:
+        assert lib.tpt_cuda_ctx_set_wait_limit(cuda.ctx, 100) == 0
+        cuda.linear_dev(x, w, None, 0, None, y)
+        with pytest.raises(OpError) as e:
+            cuda.sync()
+        assert e.value.code == 7  # TPT_TIMEOUT
+    finally:
+        assert lib.tpt_cuda_ctx_set_wait_limit(cuda.ctx, 0) == 0
+    ref = x.double() @ w.double().t()
+    bound = (k + 2) * 2.0**-23 * (x.double().abs() @ w.double().abs().t())
+    for _ in range(2):
+        cuda.linear_dev(x, w, None, 0, None, y)
+        cuda.sync()
+        check(y, ref, bound)

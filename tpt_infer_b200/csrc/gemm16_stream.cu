@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
     if (SUM || !a.ids) share(a.n, at, end);
     if (!a.ids) {
         // a dense layer's rows start towards the L2 while the kernel before it ends
-        for (int r = at + (int)threadIdx.x; r < end; r += ST_T)
+        for (int r = at + (int)threadIdx.x; r < end && a.k >= 8; r += ST_T)
             prefetch_l2_bulk(w + (size_t)r * a.ldw, (uint32_t)(a.k & ~7) * 2);
     }
     const int kch = (a.k + ST_CHUNK - 1) / ST_CHUNK;  // steps of one product
