@@ -67,16 +67,23 @@ __device__ __forceinline__ float sigmoid_score(float l) {
     return l < -87.0f ? 0.0f : fmaf(r, fmaf(-d, r, 1.0f), r);
 }
 
-// One warp per token. Each group has `lanes` (a power of two) neighbouring
-// lanes and each of them V of its experts in order, so a group's best values
-// meet in log2(lanes) exchanges, and of equal values the lowest lane's lowest
-// one is the lowest expert. The chosen experts come out one per round: the
-// warp's largest key, its first lane, that lane's next best. What it does is
-// bound by instructions, not by the 4 E bytes it reads.
+// The largest of the warp's floats (no NaN among them)
+__device__ __forceinline__ float warp_best(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// One warp per token. Each group has 2^lane_bits neighbouring lanes and each of
+// them V of its `per` experts in order, so a group's best values meet in
+// lane_bits exchanges, and of equal values the lowest lane's lowest one is the
+// lowest expert. Each lane keeps its best three in order, and the chosen experts
+// come out one per round: the warp's largest value, its first lane, that lane's
+// next best. What it does is bound by instructions, not by the 4 E bytes it reads.
 template <typename T, int V>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32)
-    k_route_experts(const T *__restrict__ logits, size_t ld, int tokens, int experts, int softmax,
-                    const float *__restrict__ bias, int groups, int groups_kept, int group_top, int lanes, int vec,
+    k_route_experts(const T *__restrict__ logits, size_t ld, int tokens, int per, int softmax,
+                    const float *__restrict__ bias, int groups, int groups_kept, int group_top, int lane_bits, int vec,
                     int bias_vec, int top_k, int renormalise, float scale, const uint8_t *__restrict__ mask, int *__restrict__ ids,
                     float *__restrict__ weights) {
     pdl_wait();
@@ -88,9 +95,9 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32)
     float w_mine = 0.0f;
     if (!mask || mask[t]) {
         const float NEG = -INFINITY;
-        const int per = experts / groups, q = lane / lanes, at0 = (lane & (lanes - 1)) * V;
-        const int n = q < groups ? min(V, per - at0) : 0;  // this lane's experts (none: n <= 0)
-        const int e0 = q * per + at0;
+        const int lanes = 1 << lane_bits, q = lane >> lane_bits, sub = lane & (lanes - 1);
+        const int n = q < groups ? min(V, per - sub * V) : 0;  // this lane's experts (none: n <= 0)
+        const int e0 = q * per + sub * V;
         const T *row = logits + (size_t)t * ld;
         float c[V];
         load_logits<T, V>(row + e0, vec, n, c);
@@ -98,7 +105,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32)
         if (softmax) {
 #pragma unroll
             for (int i = 0; i < V; i++) top = fmaxf(top, c[i]);  // NaN: the other operand
-            top = warp_max(top);
+            top = warp_best(top);
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < V; i++) {
@@ -110,7 +117,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32)
             rsum = sum > 0.0f ? __frcp_rn(sum) : 0.0f;
 #pragma unroll
             for (int i = 0; i < V; i++) c[i] = c[i] > NEG ? c[i] * rsum : NEG;
-        } else {
+        } else if (!bias) {
 #pragma unroll
             for (int i = 0; i < V; i++) c[i] = c[i] > NEG ? sigmoid_score(c[i]) : NEG;
         }
@@ -118,71 +125,78 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32)
             float bv[V];
             load_logits<float, V>(bias + e0, bias_vec, n, bv);
 #pragma unroll
-            for (int i = 0; i < V; i++) bv[i] = c[i] + bv[i];
-#pragma unroll
-            for (int i = 0; i < V; i++) c[i] = c[i] > NEG && bv[i] > NEG ? bv[i] : NEG;  // a NaN or -inf bias: off, too
+            for (int i = 0; i < V; i++) {
+                bv[i] += softmax ? c[i] : sigmoid_score(c[i]);
+                c[i] = c[i] > NEG && bv[i] > NEG ? bv[i] : NEG;  // a NaN or -inf bias: off, too
+            }
         }
-        // This lane's best two, the lower index first among equals; `gone` marks
-        // the ones already chosen.
-        float b1, b2;
-        int i1, i2;
-        using Bits = typename std::conditional<(V > 32), unsigned long long, unsigned>::type;
-        Bits gone = 0;
-        auto scan = [&]() {
-            b1 = b2 = NEG;
-            i1 = i2 = 0;
+        // This lane's best values below (from, from_i), in order, the lower index first
+        // among equals; MORE marks the last of them, behind which others may come.
+        constexpr int D = V < 3 ? V : 3, MORE = V > D ? 1 << 16 : 0;
+        float b[D];
+        int at[D];
+        auto scan = [&](bool all, float from, int from_i) {
+#pragma unroll
+            for (int d = 0; d < D; d++) {
+                b[d] = NEG;
+                at[d] = 0;
+            }
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const float v = gone >> i & 1 ? NEG : c[i];
-                const bool first = v > b1, second = v > b2;
-                i2 = first ? i1 : second ? i : i2;
-                b2 = fmaxf(b2, fminf(b1, v));
-                i1 = first ? i : i1;
-                b1 = fmaxf(b1, v);
+                const float v = all || c[i] < from || (c[i] == from && i > from_i) ? c[i] : NEG;
+                bool over[D];
+#pragma unroll
+                for (int d = 0; d < D; d++) over[d] = v > b[d];
+#pragma unroll
+                for (int d = D - 1; d > 0; d--) {
+                    at[d] = over[d - 1] ? at[d - 1] : over[d] ? i : at[d];
+                    b[d] = fmaxf(b[d], fminf(b[d - 1], v));
+                }
+                at[0] = over[0] ? i : at[0];
+                b[0] = fmaxf(b[0], v);
             }
+            at[D - 1] |= MORE;
         };
-        scan();
+        scan(true, 0.0f, 0);
         if (groups > 1) {
-            float g1 = b1, g2 = b2;
+            float g1 = b[0], g2 = D > 1 ? b[D > 1 ? 1 : 0] : NEG;
             for (int o = 1; o < lanes; o <<= 1) {
                 const float p1 = __shfl_xor_sync(0xffffffffu, g1, o), p2 = __shfl_xor_sync(0xffffffffu, g2, o);
                 g2 = fmaxf(fminf(g1, p1), fmaxf(g2, p2));
                 g1 = fmaxf(g1, p1);
             }
+            // a group's lanes share the comparisons with the other groups
             const float mine = group_top == 2 && g2 > NEG ? g1 + g2 : g1;
             int better = 0;
-            for (int g = 0; g < groups; g++) {
-                const float o = __shfl_sync(0xffffffffu, mine, g * lanes);
-                better += o > mine || (o == mine && g < q) ? 1 : 0;
+            for (int g0 = 0; g0 < groups; g0 += lanes) {
+                const int g = g0 + sub;
+                const float o = __shfl_sync(0xffffffffu, mine, (g << lane_bits) & 31);
+                better += g < groups && (o > mine || (o == mine && g < q)) ? 1 : 0;
             }
+            for (int o = 1; o < lanes; o <<= 1) better += __shfl_xor_sync(0xffffffffu, better, o);
             if (better >= groups_kept) {  // nothing of this lane can be chosen
-                b1 = b2 = NEG;
-                gone = ~(Bits)0;
+#pragma unroll
+                for (int d = 0; d < D; d++) b[d] = NEG;
             }
         }
-        int cached = 2;  // how many of (b1, b2) stand
         for (int j = 0; j < top_k; j++) {
-            const unsigned key = order_key(b1 + 0.0f);  // -0 counts as 0
-            const unsigned best = __reduce_max_sync(0xffffffffu, key);
-            if (best == order_key(NEG)) break;  // no expert is left
-            const int owner = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1;
-            const int e = __shfl_sync(0xffffffffu, e0 + i1, owner);
+            const float best = warp_best(b[0]);
+            if (best == NEG) break;  // no expert is left
+            const int owner = __ffs(__ballot_sync(0xffffffffu, b[0] == best)) - 1;
+            const int e = __shfl_sync(0xffffffffu, e0 + at[0], owner);
             if (lane == j) id_mine = e;
             if (lane == owner) {
-                gone |= (Bits)1 << i1;
-                b1 = b2;
-                i1 = i2;
-                cached--;
-            }
-            if (V > 1 && __any_sync(0xffffffffu, cached == 0)) {
-                if (cached == 0) {
-                    scan();
-                    cached = 2;
+#pragma unroll
+                for (int d = 0; d + 1 < D; d++) {
+                    b[d] = b[d + 1];
+                    at[d] = at[d + 1];
                 }
+                b[D - 1] = NEG;
             }
-            if (V == 1 && lane == owner) b1 = NEG;
+            if (MORE && (e & MORE) && lane == owner) scan(false, best, (e & (MORE - 1)) - e0);
         }
         if (id_mine >= 0) {
+            if (MORE) id_mine &= MORE - 1;
             const float l = to_f32(row[id_mine]);
             w_mine = softmax ? softmax_term(l, top) * rsum : sigmoid_score(l);
         }
@@ -203,9 +217,9 @@ void launch_route(tpt_cuda_ctx *ctx, const void *logits, size_t ld, int tokens, 
                   const float *bias, int groups, int groups_kept, int group_top, int top_k, int renormalise,
                   float scale, const uint8_t *mask, int *ids, float *weights) {
     const dim3 grid((tokens + ROUTE_WARPS - 1) / ROUTE_WARPS);
-    int lanes = 32;
-    while (lanes * groups > 32) lanes /= 2;
-    const int per = experts / groups, need = (per + lanes - 1) / lanes;
+    int lane_bits = 5;
+    while (groups << lane_bits > 32) lane_bits--;
+    const int per = experts / groups, need = (per + (1 << lane_bits) - 1) >> lane_bits;
     int v = 1;
     while (v < need) v *= 2;
     const size_t word = v * sizeof(T) < 16 ? v * sizeof(T) : 16;
@@ -213,8 +227,8 @@ void launch_route(tpt_cuda_ctx *ctx, const void *logits, size_t ld, int tokens, 
     const size_t bword = v * 4 < 16 ? v * 4 : 16;
     const bool bias_vec = per % v == 0 && ((uintptr_t)bias % bword) == 0;
     auto go = [&](auto kern) {
-        launch_pdl(kern, grid, ROUTE_WARPS * 32, 0, ctx->stream, (const T *)logits, ld, tokens, experts,
-                   score == TPT_SCORE_SOFTMAX, bias, groups, groups_kept, group_top, lanes, vec, bias_vec, top_k, renormalise,
+        launch_pdl(kern, grid, ROUTE_WARPS * 32, 0, ctx->stream, (const T *)logits, ld, tokens, per,
+                   score == TPT_SCORE_SOFTMAX, bias, groups, groups_kept, group_top, lane_bits, vec, bias_vec, top_k, renormalise,
                    scale, mask, ids, weights);
     };
     // groups <= 32 and experts <= 1024: at most 64 experts a lane (17 groups of 60)
