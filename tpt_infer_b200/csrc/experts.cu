@@ -22,12 +22,6 @@ namespace {
 
 constexpr int ROUTE_WARPS = 8;
 
-// A total order of floats as unsigned integers; NaN does not occur.
-__device__ __forceinline__ unsigned order_key(float v) {
-    const unsigned b = __float_as_uint(v);
-    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
-}
-
 // V consecutive logits; vec: as 16-, 8- or 4-byte words
 template <typename T, int V>
 __device__ __forceinline__ void load_logits(const T *p, bool vec, int n, float (&s)[V]) {
@@ -253,14 +247,14 @@ void launch_route(tpt_cuda_ctx *ctx, const void *logits, size_t ld, int tokens, 
 // Sorts the (token, choice) pairs by expert: pos[i] is pair i's slot (-1: no
 // expert), row_token[slot] its token (null: not wanted); tiles lists each
 // expert's slots in runs of at most tile_rows, an expert's runs of equal
-// length up to the step that the product kernels count columns in.
+// length up to TILE_STEP.
 // One cluster of eight blocks: each counts its share of the pairs in shared
 // memory, the blocks add one another's counts, and each places its share (65536
 // pairs of 128 experts: 9 us).
 constexpr int PLAN_T = 1024, CL = 8;
 
 __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(PLAN_T)
-    k_experts_plan(const int *__restrict__ ids, int pairs, int top_k, int experts, int tile_rows, int step, int *pos,
+    k_experts_plan(const int *__restrict__ ids, int pairs, int top_k, int experts, int tile_rows, int *pos,
                    int *row_token, Tile16 *tiles, int *n_tiles, unsigned *gflags) {
     extern __shared__ int plan_smem[];
     int *count = plan_smem, *first = plan_smem + experts;
@@ -324,7 +318,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(PLAN_T)
         if (e < experts) first[e] = at + before;
         if (rank == 0 && nt > 0) {
             int each = (total + nt - 1) / nt;
-            each = (each + step - 1) / step * step;
+            each = (each + TILE_STEP - 1) / TILE_STEP * TILE_STEP;
             for (int r = 0, k = wn + n - nt; r < nt; r++, k++) {
                 // no tile is empty: (nt - 1) * each <= (nt - 1) * tile_rows < total
                 const int place = r % TILE_RUN;
@@ -564,7 +558,7 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
         const size_t pairs = tn * top_k;
         const T *xt = x + t0 * ldx;
         launch_pdl(k_experts_plan, CL, PLAN_T, experts * 8, ctx->stream, ids + t0 * top_k, (int)pairs, (int)top_k,
-                   (int)experts, tile_rows, tile_rows == 256 ? 32 : 16, pos, tok, tiles, n_tiles, ctx->d_flags);
+                   (int)experts, tile_rows, pos, tok, tiles, n_tiles, ctx->d_flags);
         st = after_launch(ctx, "experts_plan");
         if (st) return st;
         if (!gather) {

@@ -20,6 +20,9 @@ namespace tpt {
 // An expert's tiles lie in runs of up to TILE_RUN: `run` holds the tile's place
 // in its run (from bit 8) and the run's length (8 bits).
 constexpr int TILE_RUN = 8;
+// The step in which the products count a tile's columns (with steps of 32 in place of
+// 16: 2048 tokens, 8 experts of 4096 x 11008, 2 chosen: 1280 us against 1200).
+constexpr int TILE_STEP = 16;
 struct Tile16 {
     int expert, row0, rows, run;
 };

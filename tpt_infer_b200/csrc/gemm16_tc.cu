@@ -3,7 +3,7 @@
 //
 // The weights are the MMA's M side and the tokens its N side: an expert's
 // weights stream through 128-row tiles whatever its number of tokens, and the
-// number of columns follows the tokens in steps of 16 or 32, so a short list
+// number of columns follows the tokens in steps of 16, so a short list
 // of tokens costs no padded rows of 128. A tensor-memory lane is an output
 // feature and its columns are tokens: the bias is one register, and a warp's
 // store of one column is 32 consecutive features of one row.
@@ -279,7 +279,7 @@ __device__ __forceinline__ TileAt tile_at(const Args &a, int t) {
         r.expert = q.x;
         r.row0 = q.y;
         r.rows = q.z;
-        r.cols = (q.z + 31) & ~31;
+        r.cols = (q.z + TILE_STEP - 1) & ~(TILE_STEP - 1);
     } else {
         const int ttiles = (a.rows + a.tile_n - 1) / a.tile_n;
         const int sweep = a.group * a.ftiles;
