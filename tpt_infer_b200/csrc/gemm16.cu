@@ -62,7 +62,8 @@ __device__ __forceinline__ void pad_row(uintptr_t first, uintptr_t last, uintptr
     }
 }
 
-// blockIdx.y: the operand; a warp per row
+// blockIdx.y: the operand; a warp per row. Bound by the bytes read and written (1003 and
+// 1537 rows of 2051: 21 MB, ~5 us, from L2 in part).
 __global__ void __launch_bounds__(256) k_pad_rows16(PadJob a, PadJob b, PadJob c) {
     pdl_wait();
     pdl_trigger();
