@@ -11,7 +11,7 @@
 //   k_gemm16_pair   256 weight rows x up to 256 tokens per pair of SMs
 //                   (cta_group::2), persistent, for work bound by the MMA
 //                   (8192 x 4096 x 11008, gelu: 480 us = 1540 TFLOP/s at full
-//                   clocks, 557 us = 1326 where the power limit holds them)
+//                   clocks, 555 us = 1330 where the power limit holds them)
 //   k_gemm16_split  128 weight rows x up to 128 tokens per SM, k split over a
 //                   cluster, for work bound by the weights' stream
 //                   (64 x 4096 x 11008: 92 MB in 21.3 us = 4.3 TB/s)
