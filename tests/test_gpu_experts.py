@@ -137,6 +137,26 @@ def test_route_masked_experts_and_tokens(cuda, score, groups, kept):
     run_route(cuda, l, 5, score, bias, groups, kept, 2 if groups > 1 else 1, True, 1.0, mask)
 
 
+@pytest.mark.parametrize("e,k,groups,kept", [(64, 8, 1, 1), (256, 8, 1, 1), (256, 8, 8, 4), (1000, 32, 1, 1),
+                                             (1024, 32, 4, 2), (96, 20, 2, 1)])
+def test_route_best_experts_side_by_side(cuda, e, k, groups, kept):
+    """The chosen experts lie next to one another, falling, rising, all equal, or tied in runs, anywhere in the row; and
+    several biases of +inf."""
+    import torch
+
+    l = torch.full((40, e), -3.0)
+    for t in range(40):
+        at = (t * 37) % (e - k + 1)
+        run = [torch.arange(k).flip(0), torch.arange(k), torch.zeros(k), torch.arange(k) // 4][t % 4].float()
+        l[t, at:at + k] = run / 8
+    l = l.cuda()
+    run_route(cuda, l, k, groups=groups, kept=kept)
+    bias = np.zeros(e, np.float32)
+    bias[5:5 + 6] = np.inf
+    bias[e - 2:] = np.inf
+    run_route(cuda, l, k, "sigmoid", bias, groups, kept, 2)
+
+
 def test_route_strided_rows_and_no_tokens(cuda):
     import torch
 
