@@ -473,3 +473,20 @@ def test_experts_id_past_the_last_expert_is_reported(cuda):
     ids[2, 1] = -1
     check(y, *want_experts(x, ids, wts, w_in, w_out, "silu", True, None, "bf16"))
     run_experts(cuda, x, ids, wts, w_in, w_out, "silu", True, None, "bf16")
+
+
+@pytest.mark.parametrize("t", [1, 3, 4, 40])
+@pytest.mark.parametrize("d,f", [(1, 5), (1, 203), (1003, 1)])
+def test_experts_what_lies_behind_a_single_row_stays_out(cuda, t, d, f):
+    """One expert of one output or one hidden value: the weight is a single row, with NaN right behind it."""
+    import torch
+
+    x, ids, wts, w_in, w_out = expert_inputs(t, 1, 1, d, f, "bf16", False)
+
+    def alone(w):
+        buf = torch.full((w.numel() + 64,), float("nan"), dtype=w.dtype, device="cuda")
+        v = buf[: w.numel()].view(w.shape)
+        v.copy_(w)
+        return v
+
+    run_experts(cuda, x, ids, wts, alone(w_in), alone(w_out), "relu", False, None, "bf16")

@@ -299,3 +299,55 @@ def test_linear_wait_limit_reports_a_timeout_and_the_context_recovers(cuda, m, k
         cuda.linear_dev(x, w, None, 0, None, y)
         cuda.sync()
         check(y, ref, bound)
+
+
+def behind(rows, cols, ld, dtype, fill):
+    """A [rows, cols] view, rows ld apart, into a buffer of `fill` that goes on behind its last value; the base is on
+    16 bytes."""
+    import torch
+
+    buf = torch.full((rows * ld + 64,), fill, dtype=dtype, device="cuda")
+    return buf, buf.as_strided((rows, cols), (ld, 1))
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("fill", [float("nan"), float("inf")])
+@pytest.mark.parametrize("m,n,k,ld", [(1, 70, 1003, 1008), (4, 70, 1003, 1008), (5, 70, 1003, 1008),
+                                      (3, 33, 70, 72), (2, 17, 1, 8), (4, 40, 63, 128), (1, 600, 4093, 4096),
+                                      (1, 1, 1003, 1003), (4, 1, 1003, 1003), (4, 1, 1, 1), (1, 1, 9, 9), (2, 1, 65, 65),
+                                      (200, 1, 1003, 1003), (300, 40, 1003, 1008)])
+def test_what_lies_behind_a_row_stays_out(cuda, m, n, k, ld, fill, t):
+    """Rows on 16 bytes whose length is not a multiple of 8, with NaN or infinities between and behind them, in both
+    operands: few tokens give what many give."""
+    x, w, b, r, y = inputs(m, n, k, t, True, True, t)
+    ref, bound = want(x, w, b, "none", r, t)
+    (_, xs), (_, ws) = behind(m, k, ld, x.dtype, fill), behind(n, k, ld, w.dtype, fill)
+    xs.copy_(x)
+    ws.copy_(w)
+    import torch
+
+    torch.cuda.synchronize()
+    cuda.linear_dev(xs, ws, b, 0, r, y)
+    cuda.sync()
+    check(y, ref, bound)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4])
+@pytest.mark.parametrize("n,k", [(30, 64), (264, 512), (130, 1000)])
+def test_few_tokens_with_strided_rows_on_16_bytes(cuda, m, n, k):
+    """Strided operands that are read in place: x, w, residual and y; what lies between y's rows stays."""
+    import torch
+
+    x, w, b, r, _ = inputs(m, n, k, "bf16", True, True, "f32")
+    (_, xs), (_, ws), (_, rs), (buf, ys) = (behind(m, k, k + 24, x.dtype, 3.0), behind(n, k, k + 8, w.dtype, -5.0),
+                                            behind(m, n, n + 3, r.dtype, 9.0), behind(m, n, n + 5, r.dtype, 7.0))
+    for v, src in ((xs, x), (ws, w), (rs, r)):
+        v.copy_(src)
+    ref, bound = want(x, w, b, "relu", r, "f32")
+    torch.cuda.synchronize()
+    cuda.linear_dev(xs, ws, b, 1, rs, ys)
+    cuda.sync()
+    check(ys, ref, bound)
+    if m > 1:
+        assert (buf[: m * (n + 5)].view(m, n + 5)[:, n:] == 7).all()
+    assert (buf[m * (n + 5):] == 7).all()

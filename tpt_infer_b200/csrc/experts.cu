@@ -473,13 +473,14 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
         return at;
     };
     // Weights whose rows TMA and 128-bit loads cannot read are copied first: all
-    // of them, or, for a few pairs, the named experts'.
+    // of them, or, for a few pairs, the named experts'. (A single row starts on 16
+    // bytes whatever its length, but its last load would reach past its end.)
     const T *w_src[2] = {w_in, w_out};
     const size_t w_er[2] = {(gated ? 2 : 1) * f, d}, w_k[2] = {d, f};
     bool pad[2];
     size_t o_w[2] = {0, 0};
     for (int i = 0; i < 2; i++) {
-        pad[i] = !rows16_ok(w_src[i], w_k[i], experts * w_er[i]);
+        pad[i] = w_k[i] % 8 != 0 || !rows16_ok(w_src[i], w_k[i], experts * w_er[i]);
         if (pad[i]) o_w[i] = take(experts * w_er[i] * up8(w_k[i]) * 2);
     }
     // Up to 16 tokens' hidden values keep 16 bits between the products, in two planes:

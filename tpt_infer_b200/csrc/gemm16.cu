@@ -175,7 +175,13 @@ int tpt_cuda_linear_dev(tpt_cuda_ctx *ctx, int dtype, const void *x, size_t ldx,
         if (st) return st;
         if (k == 0) g.k = 8;
     }
-    if (m <= STREAM_TOKENS && stream_x_bytes(m, (size_t)g.k) <= STREAM_X_BYTES) return launch_gemm16_stream(ctx, dtype, g);
+    // The stream kernel reads weights eight at a time: past k the rows must hold the
+    // copy's zeros, not what lies between strided rows or behind a single one (the
+    // other kernels' maps end at k; 1 x 4096 x 4093 in rows of 4096: 9.8 us there, 18.4
+    // copied first).
+    const bool whole = k % 8 == 0 || pw;
+    if (m <= STREAM_TOKENS && whole && stream_x_bytes(m, (size_t)g.k) <= STREAM_X_BYTES)
+        return launch_gemm16_stream(ctx, dtype, g);
     return launch_gemm16(ctx, dtype, g);
 }
 

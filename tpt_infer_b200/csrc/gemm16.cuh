@@ -58,7 +58,8 @@ struct Gemm16 {
 // must pass rows16_ok (the copies below make them).
 int launch_gemm16(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g);
 
-// The kernels of a few tokens, for operands like launch_gemm16's: a dense product of
+// The kernels of a few tokens, for operands like launch_gemm16's whose weight rows hold
+// k values and then zeros up to a multiple of 8: a dense product of
 // up to STREAM_TOKENS rows, and both of the experts' products of as many tokens and
 // up to STREAM_PAIRS (token, choice) pairs. `in` reads the tokens' rows and writes
 // [tile][4][2][ldy], one tile per distinct expert; `out` reads those and writes the

@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
 #pragma unroll
                     for (int s = 0; s < 2; s++) {
                         const int k0 = (kc + d) * ST_CHUNK + 32 * s;
-                        const bool in = kc + d < last && k0 + 8 * t < a.k;
+                        const bool in = kc + d < last && k0 + 8 * t < a.k;  // zeros from k to the word's end
                         const size_t o = h * half + (size_t)k0;
                         buf[d][h * 4 + s] = load8(p0 + o, row0 && in);
                         buf[d][h * 4 + 2 + s] = load8(p1 + o, row1 && in);
