@@ -351,3 +351,22 @@ def test_few_tokens_with_strided_rows_on_16_bytes(cuda, m, n, k):
     if m > 1:
         assert (buf[: m * (n + 5)].view(m, n + 5)[:, n:] == 7).all()
     assert (buf[m * (n + 5):] == 7).all()
+
+
+@pytest.mark.parametrize("m,n", [(1, 3), (4, 4), (5, 130), (100, 40), (300, 257)])
+@pytest.mark.parametrize("ld", [0, 1, 64, 4096])
+def test_no_products_with_null_operands_and_any_stride(cuda, m, n, ld):
+    """k = 0 through the C ABI: x and w may be null, whatever their strides say: act(bias) + residual."""
+    import torch
+
+    from tpt_infer_b200._capi import lib
+
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+    b = torch.randn(n, generator=g, device="cuda").bfloat16()
+    r = torch.randn(m, n, generator=g, device="cuda")
+    y = torch.full((m, n), float("nan"), device="cuda")
+    p = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+    torch.cuda.synchronize()
+    assert lib.tpt_cuda_linear_dev(cuda.ctx, 2, None, ld, m, 0, None, ld, n, p(b), 1, p(r), n, p(y), n, 0) == 0
+    cuda.sync()
+    assert torch.equal(y, b.float().clamp(min=0) + r)

@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(256) k_pad_rows16(PadJob a, PadJob b, PadJob c
         rows = __popc(firsts) * er;
     }
     const size_t pieces = k ? (k + 7) / 8 : 1;
-    const uintptr_t first = reinterpret_cast<uintptr_t>(src), last = first + ((all - 1) * ld + k) * 2;
+    // an operand without values (k = 0) may be a null pointer with any stride: no word lies inside it
+    const uintptr_t first = reinterpret_cast<uintptr_t>(src), last = first + (k ? ((all - 1) * ld + k) * 2 : 0);
     for (size_t i = blockIdx.x * (size_t)8 + (threadIdx.x >> 5); i < rows; i += (size_t)gridDim.x * 8) {
         size_t r = i;
         if (ids) {
