@@ -370,3 +370,38 @@ def test_no_products_with_null_operands_and_any_stride(cuda, m, n, ld):
     assert lib.tpt_cuda_linear_dev(cuda.ctx, 2, None, ld, m, 0, None, ld, n, p(b), 1, p(r), n, p(y), n, 0) == 0
     cuda.sync()
     assert torch.equal(y, b.float().clamp(min=0) + r)
+
+
+def runs_out_and_recovers(cuda, m, k, n, act=0):
+    """A launch under a wait limit of 100 cycles is reported as a timeout; with the default limit the next are right."""
+    import torch
+
+    from tpt_infer_b200 import OpError
+    from tpt_infer_b200._capi import lib
+
+    x, w, b, r, y = inputs(m, n, k, "bf16", True, True, "bf16")
+    flush = torch.empty(64 << 20, device="cuda")  # the operands' loads come from memory
+    flush.zero_()
+    torch.cuda.synchronize()
+    try:
+        assert lib.tpt_cuda_ctx_set_wait_limit(cuda.ctx, 100) == 0
+        cuda.linear_dev(x, w, b, act, r, y)
+        with pytest.raises(OpError) as e:
+            cuda.sync()
+        assert e.value.code == 7  # TPT_TIMEOUT
+    finally:
+        assert lib.tpt_cuda_ctx_set_wait_limit(cuda.ctx, 0) == 0
+    ref, bound = want(x, w, b, "none", r, "bf16")
+    for _ in range(2):
+        y.fill_(float("nan"))
+        torch.cuda.synchronize()
+        cuda.linear_dev(x, w, b, act, r, y)
+        cuda.sync()
+        check(y, ref, bound)
+
+
+@pytest.mark.parametrize("m,k,n", [(16, 64, 16384), (16, 128, 4096), (32, 192, 8192), (64, 256, 4096), (40, 512, 600)])
+def test_linear_wait_limit_with_every_stage_issued(cuda, m, k, n):
+    """k so short that all its copies are on their way when the products' wait runs out: they arrive before the CTAs
+    leave."""
+    runs_out_and_recovers(cuda, m, k, n)

@@ -617,6 +617,7 @@ __global__ void __launch_bounds__(S_THREADS, 2)
     }
     const int all_kb = (a.k + BK - 1) / BK;
     const int kb0 = all_kb * rank / KS, kb1 = all_kb * (rank + 1) / KS;  // KS <= all_kb
+    int issued = 0;  // the producer's stages
     if (rows > 0) {  // the same for every CTA of the cluster
         if (warp == 0) {
             // ---------------- producer ----------------
@@ -628,12 +629,10 @@ __global__ void __launch_bounds__(S_THREADS, 2)
                     r4[i] = __ldcg(a.row_token + row0 + (c < rows ? c : 0));
                 }
             }
-            bool ok = true;
-            int stage = 0, issued = 0;
+            int stage = 0;
             uint32_t phase = 0;
             for (int kb = kb0; kb < kb1; kb++) {
-                ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_p, a.gflags, true);
-                if (!ok) break;
+                if (!warp_wait(empty_bar(stage), phase ^ 1u, abort_p, a.gflags, true)) break;
                 const uint32_t w_dst = ring + stage * Cfg::STAGE_BYTES, x_dst = w_dst + W_BYTES;
                 const uint32_t fb = full_bar(stage);
                 if (elect_one()) {
@@ -656,16 +655,6 @@ __global__ void __launch_bounds__(S_THREADS, 2)
                 if (++stage == S) {
                     stage = 0;
                     phase ^= 1u;
-                }
-            }
-            if (!ok) {  // aborting: no copy stays in flight
-                const int n = issued < S ? issued : S;
-                for (int i = 0; i < n; i++) {
-                    if (--stage < 0) {
-                        stage = S - 1;
-                        phase ^= 1u;
-                    }
-                    warp_wait(full_bar(stage), phase, abort_p, a.gflags, false);
                 }
             }
         } else if (warp == 1) {
@@ -775,6 +764,11 @@ __global__ void __launch_bounds__(S_THREADS, 2)
     }
     tc_fence_before();
     __syncthreads();
+    // An aborting CTA leaves no copy in flight behind it, whichever role gave up (the
+    // MMA issuer may do so when every stage has been issued).
+    if (warp == 0 && abort_flag)
+        for (int i = max(0, issued - S); i < issued; i++)
+            warp_wait(full_bar(i % S), (uint32_t)(i / S) & 1u, abort_p, a.gflags, false);
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)Cfg::TMEM_COLS)
