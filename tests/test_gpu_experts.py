@@ -490,3 +490,28 @@ def test_experts_what_lies_behind_a_single_row_stays_out(cuda, t, d, f):
         return v
 
     run_experts(cuda, x, ids, wts, alone(w_in), alone(w_out), "relu", False, None, "bf16")
+
+
+@pytest.mark.parametrize("t,e,k,d,f", [(600, 2, 2, 776, 1032), (60, 4, 4, 2048, 264), (40, 16, 2, 1024, 520)])
+def test_experts_wait_limit_reports_a_timeout_and_the_context_recovers(cuda, t, e, k, d, f):
+    """Tiles of 256, 32 and 16 tokens under a wait limit of 100 cycles: a timeout, then right again."""
+    import torch
+
+    from tpt_infer_b200 import OpError
+    from tpt_infer_b200._capi import lib
+
+    x, ids, wts, w_in, w_out = expert_inputs(t, e, k, d, f, "bf16", True)
+    y = torch.empty_like(x)
+    flush = torch.empty(64 << 20, device="cuda")  # the operands' loads come from memory
+    flush.zero_()
+    torch.cuda.synchronize()
+    try:
+        assert lib.tpt_cuda_ctx_set_wait_limit(cuda.ctx, 100) == 0
+        cuda.experts_mlp_dev(x, ids, wts, w_in, w_out, 3, True, None, y)
+        with pytest.raises(OpError) as err:
+            cuda.sync()
+        assert err.value.code == 7  # TPT_TIMEOUT
+    finally:
+        assert lib.tpt_cuda_ctx_set_wait_limit(cuda.ctx, 0) == 0
+    for _ in range(2):
+        run_experts(cuda, x, ids, wts, w_in, w_out, "silu", True, None, "bf16")

@@ -405,3 +405,9 @@ def test_linear_wait_limit_with_every_stage_issued(cuda, m, k, n):
     """k so short that all its copies are on their way when the products' wait runs out: they arrive before the CTAs
     leave."""
     runs_out_and_recovers(cuda, m, k, n)
+
+
+@pytest.mark.parametrize("m,k,n", [(300, 4096, 2048), (1000, 128, 600), (200, 64, 16384), (2000, 776, 5000)])
+def test_linear_wait_limit_in_the_pair_kernel(cuda, m, k, n):
+    """More than 128 tokens: the SM pairs leave with their two producers at any stages, and the next call is right."""
+    runs_out_and_recovers(cuda, m, k, n)

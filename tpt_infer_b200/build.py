@@ -56,7 +56,8 @@ def _newest(paths):
 def build(force: bool = False, verbose_ptxas: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
-    headers = glob.glob(os.path.join(CSRC, "*.cuh")) + [os.path.join(ROOT, "include", "tpt_cuda.h")]
+    headers = (glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) +
+               [os.path.join(ROOT, "include", "tpt_cuda.h")])
     hdr_time = _newest(headers)
     objs = []
     jobs = []

@@ -25,6 +25,7 @@
 // drained (bounded), tensor memory is freed and the kernel returns.
 
 #include "gemm16.cuh"
+#include "pair_settle.h"
 
 namespace tpt {
 namespace {
@@ -146,6 +147,18 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_
             " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
             "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
             : "memory");
+}
+// counts `bytes` on this CTA's barrier as a copy of that size would
+__device__ __forceinline__ void mbar_complete_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t cluster_addr, int v) {
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ int ld_cluster(uint32_t cluster_addr) {
+    int v;
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+    return v;
 }
 // f32 accumulator, both operands K-major of type fmt, M x N
 __device__ __forceinline__ uint32_t idesc_f16(uint32_t fmt, uint32_t m, uint32_t n) {
@@ -298,6 +311,30 @@ __device__ __forceinline__ TileAt tile_at(const Args &a, int t) {
     return r;
 }
 
+// X's box of a tile of cols tokens, half of them a CTA's, and the bytes of one CTA's stage
+__device__ __forceinline__ int pair_box(int cols) { return cols > 128 ? 0 : cols > 64 ? 1 : 2; }
+__device__ __forceinline__ uint32_t pair_cta_bytes(int cols) { return W_BYTES + (W_BYTES >> pair_box(cols)); }
+
+// An aborting pair leaves no copy in flight behind it. Its two producers (the leader's
+// issued `mine` stages, the other `theirs`) may have stopped at different ones; the
+// leader evens out the counts of its full barriers (pair_settle.h) and waits, bounded,
+// for the copies of both. Out of line: the kernels' usual end stays short.
+__device__ __noinline__ void pair_drain(const Args &a, uint32_t full_bars, int mine, int theirs, int cluster,
+                                        int nclusters, volatile int *abort_p) {
+    const int last = max(mine, theirs), kblocks = (a.k + BK - 1) / BK;
+    for (int i = max(0, last - P_STAGES); i < last; i++) {
+        const uint32_t bar = full_bars + 8u * (i % P_STAGES);
+        const PairSettle p =
+            pair_settle(i, mine, theirs, pair_cta_bytes(tile_at(a, cluster + i / kblocks * nclusters).cols));
+        if (elect_one()) {
+            if (p.arrive) mbar_arrive_expect_tx(bar, p.expect);
+            if (p.complete) mbar_complete_tx(bar, p.complete);
+        }
+        __syncwarp();
+        warp_wait(bar, (uint32_t)(i / P_STAGES) & 1u, abort_p, a.gflags, false);
+    }
+}
+
 template <typename T, typename TY, bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     k_gemm16_pair(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ XMaps tmX,
@@ -305,6 +342,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     constexpr int S = P_STAGES;
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag;
+    __shared__ int pair_abort, pair_issued;  // a CTA of the pair gave up; stages that this CTA's producer issued
     __shared__ uint32_t tmem_slot;
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t bars = ring + S * P_STAGE_BYTES;
@@ -321,7 +359,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     const int kblocks = (a.k + BK - 1) / BK;
 
     if (threadIdx.x == 0) {
-        abort_flag = 0;
+        abort_flag = pair_abort = 0;
         for (int s = 0; s < S; s++) {
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
@@ -360,8 +398,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         for (int t = cluster; t < ntiles && ok; t += nclusters) {
             const TileAt tl = tile_at(a, t);
             const int half = tl.cols >> 1;
-            const int box = half > 64 ? 0 : half > 32 ? 1 : 2;
-            const uint32_t bytes = 2u * (W_BYTES + (W_BYTES >> box));
+            const int box = pair_box(tl.cols);
+            const uint32_t bytes = 2u * pair_cta_bytes(tl.cols);
             const int xrow = tl.row0 + (int)rank * half;
             const CUtensorMap *xmap = &tmX.box[box];
             for (int kb = 0; kb < kblocks; kb++) {
@@ -393,19 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
                 }
             }
         }
-        // an aborting pair leaves no copy in flight behind it: the leader waits
-        // (bounded) for the stages it announced and did not see consumed
-        if (!ok && leader) {
-            const int n = issued < S ? issued : S;
-            for (int i = 0; i < n; i++) {
-                if (--stage < 0) {
-                    stage = S - 1;
-                    phase ^= 1u;
-                }
-                // (it gives up with the first that never fills: the other CTA stopped too)
-                if (!warp_wait(full_bar(stage), phase, abort_p, a.gflags, false)) break;
-            }
-        }
+        if (lane == 0) pair_issued = issued;
     } else if (warp == 1) {
         if (leader) {
             // ---------------- MMA issuer ----------------
@@ -512,7 +538,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     // both CTAs stay until neither needs the other's memory or barriers
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x < 2 && abort_flag) st_cluster(map_to_rank(smem_u32(&pair_abort), threadIdx.x), 1);
+    __syncwarp();
     cluster_sync();
+    if (pair_abort) {  // the same in both
+        if (leader && warp == 0)
+            pair_drain(a, bars, pair_issued, ld_cluster(map_to_rank(smem_u32(&pair_issued), 1)), cluster, nclusters,
+                       abort_p);
+        __syncwarp();
+        cluster_sync();
+    }
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
