@@ -515,3 +515,71 @@ def test_experts_wait_limit_reports_a_timeout_and_the_context_recovers(cuda, t, 
         assert lib.tpt_cuda_ctx_set_wait_limit(cuda.ctx, 0) == 0
     for _ in range(2):
         run_experts(cuda, x, ids, wts, w_in, w_out, "silu", True, None, "bf16")
+
+
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("t,k,d,f", [(1, 3, 136, 72), (2, 8, 264, 40), (3, 3, 51, 33), (4, 8, 136, 72)])
+def test_experts_few_tokens_repeated_choices(cuda, t, k, d, f, gated):
+    """A token that names an expert two or more times takes it with each of its weights, beside tokens that name it
+    once, that share all their experts, or that name none."""
+    import torch
+
+    for seed in range(6):
+        x, ids, wts, w_in, w_out = expert_inputs(t, 12, k, d, f, "bf16", gated, seed=seed)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        ids.copy_(torch.randint(-1, [1, 2, 3, 12, 12, 12][seed], ids.shape, generator=g, device="cuda"))
+        if seed == 4:
+            ids[:] = 7
+        if seed == 5:
+            ids[t - 1] = -1
+        wts.copy_(torch.randn(wts.shape, generator=g, device="cuda"))  # of either sign
+        run_experts(cuda, x, ids, wts, w_in, w_out, "silu", gated, torch.randn_like(x) if seed % 2 else None, "bf16")
+
+
+@pytest.mark.parametrize("t", [1, 4])
+@pytest.mark.parametrize("bad", [6, 4096, 2**31 - 1])
+def test_experts_few_tokens_id_past_the_last_expert_is_reported(cuda, t, bad):
+    import torch
+
+    from tpt_infer_b200 import OpError
+
+    for d, f in ((32, 16), (33, 17)):  # read in place, and copied first
+        x, ids, wts, w_in, w_out = expert_inputs(t, 6, 3, d, f, "bf16", True)
+        ids[t - 1, 1] = bad
+        y = torch.empty_like(x)
+        torch.cuda.synchronize()
+        cuda.experts_mlp_dev(x, ids, wts, w_in, w_out, 3, True, None, y)
+        with pytest.raises(OpError) as e:
+            cuda.sync()
+        assert e.value.code == 9  # TPT_DEVICE_CHECK
+        ids[t - 1, 1] = -1
+        check(y, *want_experts(x, ids, wts, w_in, w_out, "silu", True, None, "bf16"))
+        run_experts(cuda, x, ids, wts, w_in, w_out, "silu", True, None, "bf16")
+
+
+@pytest.mark.parametrize("t", [1, 2, 4, 5])
+@pytest.mark.parametrize("d,f,pad", [(72, 40, 8), (72, 40, 3), (136, 64, 24), (75, 33, 5)])
+def test_experts_few_tokens_strided_rows(cuda, t, d, f, pad):
+    """Strided x and out with the residual in place; NaN between x's rows stays out, what lies between out's stays."""
+    import torch
+
+    x, ids, wts, w_in, w_out = expert_inputs(t, 5, 2, d, f, "f16", True)
+    xs = torch.full((t, d + pad), float("nan"), dtype=torch.float16, device="cuda")[:, :d]
+    xs.copy_(x)
+    out = torch.full((t, d + pad), 5.0, dtype=torch.float16, device="cuda")
+    r = torch.randn_like(x)
+    out[:, :d] = r
+    torch.cuda.synchronize()
+    cuda.experts_mlp_dev(xs, ids, wts, w_in, w_out, 3, True, out[:, :d], out[:, :d])
+    cuda.sync()
+    check(out[:, :d], *want_experts(x, ids, wts, w_in, w_out, "silu", True, r, "f16"))
+    assert (out[:, d:] == 5).all()
+
+
+@pytest.mark.parametrize("t", [1, 7, 8, 9, 600])
+def test_route_around_a_blocks_tokens(cuda, t):
+    """One warp a token and eight tokens a block: one token, a block less one, a full one and one more, many blocks;
+    aligned rows, and strided ones off every word."""
+    run_route(cuda, grid_logits(t, 256, t, "bf16"), 8, groups=8, kept=4, group_top=2)
+    run_route(cuda, grid_logits(t, 80, 9, "bf16")[:, 5:75], 6)
+    run_route(cuda, grid_logits(t, 80, 9, "f32")[:, 4:76], 3, groups=2, kept=1)
