@@ -583,3 +583,19 @@ def test_route_around_a_blocks_tokens(cuda, t):
     run_route(cuda, grid_logits(t, 256, t, "bf16"), 8, groups=8, kept=4, group_top=2)
     run_route(cuda, grid_logits(t, 80, 9, "bf16")[:, 5:75], 6)
     run_route(cuda, grid_logits(t, 80, 9, "f32")[:, 4:76], 3, groups=2, kept=1)
+
+
+@pytest.mark.parametrize("ty", ["bf16", "f16"])
+@pytest.mark.parametrize("t,e,k,d,f", [(3, 64, 4, 512, 200), (16, 64, 4, 512, 200), (12, 8, 8, 512, 200), (16, 2, 1, 520, 264),
+                                       (11, 1, 1, 1000, 77), (16, 8, 8, 136, 72), (5, 4, 4, 12000, 40)])
+def test_experts_up_to_16_tokens_keep_the_hidden_values_bits(cuda, t, e, k, d, f, ty):
+    """However few experts share them: the error is the last rounding's. The hidden values' second plane leaves 2^-16 of
+    each at most (bf16; f16 2^-22, and 2^-24 absolutely), the f32 sums some 2^-20: under 3 % of the rounding's own
+    error, which is taken from the rounded 64-bit result. With hidden values of one plane it is 1.2 to 1.4 times that."""
+    import torch
+
+    x, ids, wts, w_in, w_out = expert_inputs(t, e, k, d, f, ty, True)
+    y = run_experts(cuda, x, ids, wts, w_in, w_out, "silu", True, None, ty)
+    ref, _ = want_experts(x, ids, wts, w_in, w_out, "silu", True, None, ty)
+    off, least = (y.double() - ref).norm(), (ref.to(y.dtype).double() - ref).norm()
+    assert off <= 1.03 * least, float(off / least)

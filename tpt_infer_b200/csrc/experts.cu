@@ -455,7 +455,7 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
     // tiles of 16 / 32 / 256: 64 tokens (mean 4) 178 / 182 / 193, 256 tokens (16) 220 /
     // 210 / 225, 512 tokens (32) 305 / 239 / 233, 2048 tokens (128) 862 / 494 / 311.
     const size_t mean = (tokens * top_k + experts - 1) / experts;
-    const int tile_rows = mean <= 10 ? 16 : mean <= 24 ? 32 : 256;
+    const int tile_rows = mean <= 10 || tokens <= 16 ? 16 : mean <= 24 ? 32 : 256;
     // A few tokens: no plan, no slots, one tile per chosen expert (128 experts of
     // 2048 x 768, 8 chosen: 1 token 22 us against 29, 4 tokens 57 against 58; 8 tokens of
     // 64 experts, 4 chosen: 30 against 24).
