@@ -459,7 +459,8 @@ int tpt_cuda_route_experts_dev(tpt_cuda_ctx *ctx, const void *logits, int dtype,
  * tpt_cuda_route_experts_dev writes them (a negative id is no expert; an id
  * past the last expert counts as none and makes the next synchronising call
  * return TPT_DEVICE_CHECK). h is rounded to the operands' type between the
- * two products (a call of few tokens may keep what the rounding left, too); the
+ * two products (a call of few tokens, or of few values of h in all, keeps what
+ * the rounding left, too); the
  * sum over j is in f32, in a fixed order. */
 #define TPT_EXPERTS_MAX 4096
 int tpt_cuda_experts_mlp_dev(tpt_cuda_ctx *ctx, int dtype, const void *x, size_t ldx, size_t tokens, size_t d,

@@ -599,3 +599,18 @@ def test_experts_up_to_16_tokens_keep_the_hidden_values_bits(cuda, t, e, k, d, f
     ref, _ = want_experts(x, ids, wts, w_in, w_out, "silu", True, None, ty)
     off, least = (y.double() - ref).norm(), (ref.to(y.dtype).double() - ref).norm()
     assert off <= 1.03 * least, float(off / least)
+
+
+@pytest.mark.parametrize("ty", ["bf16", "f16"])
+@pytest.mark.parametrize("t,e,k,d,f", [(17, 2, 1, 256, 64), (17, 8, 3, 256, 65), (40, 16, 8, 1000, 200), (100, 3, 2, 264, 72),
+                                       (128, 2, 1, 256, 64), (256, 2, 1, 136, 32)])
+def test_experts_of_few_hidden_values_keep_their_bits(cuda, t, e, k, d, f, ty):
+    """More than 16 tokens with narrow experts: as for up to 16 tokens, the error is the last rounding's. With hidden
+    values of one plane it is 1.41 times that on average, and up to 1.6 times where few of them carry the result."""
+    import torch
+
+    x, ids, wts, w_in, w_out = expert_inputs(t, e, k, d, f, ty, True)
+    y = run_experts(cuda, x, ids, wts, w_in, w_out, "silu", True, None, ty)
+    ref, _ = want_experts(x, ids, wts, w_in, w_out, "silu", True, None, ty)
+    off, least = (y.double() - ref).norm(), (ref.to(y.dtype).double() - ref).norm()
+    assert off <= 1.03 * least, float(off / least)

@@ -455,7 +455,17 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
     // tiles of 16 / 32 / 256: 64 tokens (mean 4) 178 / 182 / 193, 256 tokens (16) 220 /
     // 210 / 225, 512 tokens (32) 305 / 239 / 233, 2048 tokens (128) 862 / 494 / 311.
     const size_t mean = (tokens * top_k + experts - 1) / experts;
-    const int tile_rows = mean <= 10 || tokens <= 16 ? 16 : mean <= 24 ? 32 : 256;
+    // Calls of few hidden values keep 16 bits of them between the products, in two planes:
+    // how the largest of them happen to round would show in the results, in up to 1.6
+    // times the error of one rounded y. Over many values that settles at 1.41, with a
+    // spread of about 1.8 / sqrt(tokens f): 0.02 from 8192 values on. The planes need tiles
+    // of 16 tokens, which leave the MMAs idle. In place of one plane in longer tiles: 12
+    // tokens, 8 of 8 experts of 2048 x 768, 30.3 -> 27.7 us; 32 tokens, 2 of 2 of 4096 x 256,
+    // 30.0 -> 18.5; 256 tokens, 2 of 8 of 4096 x 32, 35.5 -> 31. (More tokens have so few
+    // values only where f is under 32, and take longer: 1024 of f = 8 62 -> 76. 64 tokens, 8
+    // of 128 of 2048 x 768, would take 5 % longer.)
+    const bool few = tokens <= 16 || (tokens <= 256 && tokens * f <= 8192);
+    const int tile_rows = few || mean <= 10 ? 16 : mean <= 24 ? 32 : 256;
     // A few tokens: no plan, no slots, one tile per chosen expert (128 experts of
     // 2048 x 768, 8 chosen: 1 token 22 us against 29, 4 tokens 57 against 58; 8 tokens of
     // 64 experts, 4 chosen: 30 against 24).
@@ -483,11 +493,7 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
         pad[i] = w_k[i] % 8 != 0 || !rows16_ok(w_src[i], w_k[i], experts * w_er[i]);
         if (pad[i]) o_w[i] = take(experts * w_er[i] * up8(w_k[i]) * 2);
     }
-    // Up to 16 tokens' hidden values keep 16 bits between the products, in two planes:
-    // their results come from few values, and how the largest of them happen to round
-    // would show (up to 1.55 times the error of one rounded y; many tokens' average to
-    // 1.41). The products have the MMAs idle; 64 tokens would take 5 % longer.
-    const int planes = tile_rows == 16 && tokens <= 16 ? 2 : 1;
+    const int planes = few ? 2 : 1;
     const size_t per_token = top_k * (planes * ldh * 2 + ldp * 4 + (gather ? 0 : lds * 2) + 8);
     size_t chunk = EXPERTS_WS_BYTES / per_token;
     if (chunk < 1) chunk = 1;
