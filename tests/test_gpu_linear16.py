@@ -411,3 +411,32 @@ def test_linear_wait_limit_with_every_stage_issued(cuda, m, k, n):
 def test_linear_wait_limit_in_the_pair_kernel(cuda, m, k, n):
     """More than 128 tokens: the SM pairs leave with their two producers at any stages, and the next call is right."""
     runs_out_and_recovers(cuda, m, k, n)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("m", [1, 4, 40, 300])
+def test_smooth_activations_left_of_zero(cuda, m, out, act):
+    """The left tails, relatively. y = x / (1 + e^-z), z = x (silu) or 2 sqrt(2/pi) (x + 0.044715 x^3) (gelu, within
+    2 |z| 2^-23 relatively for its roundings and its constants'). f32: expf's 2 ulp, the sum's, the reciprocal's and the
+    product's roundings, under 5 * 2^-23. bf16: the hardware exponential's documented 2 + 1.173 |z| ulp, 4 for the rest,
+    and the last rounding."""
+    import torch
+
+    z = -torch.linspace(0.01, 85, 1000, dtype=torch.float64)
+    v = z if act == "silu" else -torch.linspace(0.01, 10, 1000, dtype=torch.float64)
+    v = v.bfloat16().cuda()
+    x = torch.zeros(m, 8, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(1000, 8, dtype=torch.bfloat16, device="cuda")
+    x[:, 0], w[:, 0] = 1, v
+    y = torch.empty(m, 1000, dtype=_types()[out], device="cuda")
+    torch.cuda.synchronize()
+    cuda.linear_dev(x, w, None, ACTS[act], None, y)
+    cuda.sync()
+    v = v.double()
+    z = v if act == "silu" else 2 * (2 / torch.pi) ** 0.5 * (v + 0.044715 * v**3)
+    ref = v * torch.sigmoid(z)
+    own = 0 if act == "silu" else 2 * z.abs()
+    rel = (5 + own) * 2.0**-23 if out == "f32" else (6 + own + 1.173 * z.abs()) * 2.0**-23 + 1.01 * 2.0**-8
+    d = (y.double() - ref).abs() / ref.abs()
+    assert (d <= rel).all(), (float(d.max() * 2**23), float((d / rel).max()))

@@ -128,27 +128,38 @@ __device__ __forceinline__ __half from_f32<__half>(float v) {
 // weight makes the first what it is and the second an infinity of any sign, or 0 x inf.
 __device__ __forceinline__ float add_low(float upper, float lower) { return isfinite(upper) ? upper + lower : upper; }
 
-// The activations of the 16-bit products' epilogues, C values in place; act is
-// uniform, so the choice is one branch for all of them. Both smooth ones are
-// x / (1 + e^-z) with the hardware's exponential and quotient (errors of a few
-// 2^-22, far under the 16-bit rounding that follows): z = x for silu, and
-// z = 2 sqrt(2 / pi) (x + 0.044715 x^3) for gelu, since
-// 0.5 (1 + tanh(z / 2)) = 1 / (1 + e^-z). Far left e^-z is +inf and the
-// quotient -0, the limit. relu leaves NaN a NaN.
-template <int C>
+// x / (1 + e^-z). HARD takes the hardware's exponential and quotient: a relative error of
+// (6 + 1.2 |z|) 2^-23, since the exponential's grows with its argument (under 2^-16 at
+// z = -80), far under the rounding to 16 bits that follows; left of -87 the quotient may be
+// -0, its limit. Otherwise, for f32 results, expf(-|z|), which left of zero is the numerator
+// too, and the hardware's reciprocal with one Newton step: 5 * 2^-23 down to the smallest
+// normal results.
+template <bool HARD>
+__device__ __forceinline__ float over_one_plus_exp(float x, float z) {
+    if (HARD) return __fdividef(x, 1.0f + __expf(-z));
+    const float e = expf(-fabsf(z)), d = 1.0f + e;
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    r = fmaf(r, fmaf(-d, r, 1.0f), r);
+    return x * (z < 0.0f ? e * r : r);
+}
+
+// The activations of the products' epilogues, C values in place, HARD as above; act is
+// uniform, so the choice is one branch for all of them. silu has z = x, and gelu
+// z = 2 sqrt(2 / pi) (x + 0.044715 x^3), since 0.5 (1 + tanh(z / 2)) = 1 / (1 + e^-z); z's
+// own roundings add 2 |z| 2^-23 to the relative error. relu leaves NaN a NaN.
+template <bool HARD, int C>
 __device__ __forceinline__ void act16(float (&v)[C], int act) {
     if (act == TPT_ACT_RELU) {
 #pragma unroll
         for (int i = 0; i < C; i++) v[i] = v[i] < 0.0f ? 0.0f : v[i];
     } else if (act == TPT_ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < C; i++) {
-            const float z = v[i] * fmaf(0.0713548162726f * v[i], v[i], 1.5957691216057f);
-            v[i] = __fdividef(v[i], 1.0f + __expf(-z));
-        }
+        for (int i = 0; i < C; i++)
+            v[i] = over_one_plus_exp<HARD>(v[i], v[i] * fmaf(0.0713548162726f * v[i], v[i], 1.5957691216057f));
     } else if (act == TPT_ACT_SILU) {
 #pragma unroll
-        for (int i = 0; i < C; i++) v[i] = __fdividef(v[i], 1.0f + __expf(-v[i]));
+        for (int i = 0; i < C; i++) v[i] = over_one_plus_exp<HARD>(v[i], v[i]);
     }
 }
 

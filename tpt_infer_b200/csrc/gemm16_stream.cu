@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
             }
             if (SUM) v[0] = add_low(v[0], rest);
             if (a.bias) v[0] += to_f32(static_cast<const T *>(a.bias)[g_f + r]);
-            act16(v, a.act);
+            act16<!std::is_same<TY, float>::value>(v, a.act);
             if (GATED) v[0] *= u;
             if (a.residual) v[0] += to_f32(static_cast<const TY *>(a.residual)[(size_t)o * a.ldr + g_f + r]);
             if (a.ids && !SUM) {

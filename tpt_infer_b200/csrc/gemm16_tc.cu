@@ -209,7 +209,7 @@ __device__ __forceinline__ void epilogue16(const Args &a, float (&v)[C], const T
     const int n = f < a.n ? rows - col0 : 0;
 #pragma unroll
     for (int i = 0; i < C; i++) v[i] += b;
-    act16(v, a.act);
+    act16<!std::is_same<TY, float>::value>(v, a.act);
     if (a.residual) {
 #pragma unroll
         for (int i = 0; i < C; i++) v[i] += to_f32(rv[i]);
@@ -238,7 +238,7 @@ __device__ __forceinline__ void epilogue16_gated(const Args &a, const float (&v)
         g[i] = hi ? got : v[i];
         u[i] = hi ? v[C / 2 + i] : got;
     }
-    act16(g, a.act);
+    act16<true>(g, a.act);
     const int c0 = col0 + (hi ? C / 2 : 0);
     TY *y = static_cast<TY *>(a.y) + (row0 + c0) * a.ldy + f;
     const int n = f < a.n ? rows - c0 : 0;
