@@ -460,8 +460,11 @@ int tpt_cuda_route_experts_dev(tpt_cuda_ctx *ctx, const void *logits, int dtype,
  * past the last expert counts as none and makes the next synchronising call
  * return TPT_DEVICE_CHECK). h is rounded to the operands' type between the
  * two products (a call of few tokens, or of few values of h in all, keeps what
- * the rounding left, too); the
- * sum over j is in f32, in a fixed order. */
+ * the rounding left, too); the sum over j is in f32, in a fixed order.
+ * Workspace: weights whose rows do not start on 16 bytes (a d or f that is no
+ * multiple of 8) are copied there on each call. A call of up to 4 tokens and 32
+ * choices has room there for the experts it names, others for all of them; the
+ * workspace's size is a power of two, kept until the context is destroyed. */
 #define TPT_EXPERTS_MAX 4096
 int tpt_cuda_experts_mlp_dev(tpt_cuda_ctx *ctx, int dtype, const void *x, size_t ldx, size_t tokens, size_t d,
                              const int32_t *ids, const float *weights, size_t top_k, const void *w_in,

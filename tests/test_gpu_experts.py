@@ -614,3 +614,25 @@ def test_experts_of_few_hidden_values_keep_their_bits(cuda, t, e, k, d, f, ty):
     ref, _ = want_experts(x, ids, wts, w_in, w_out, "silu", True, None, ty)
     off, least = (y.double() - ref).norm(), (ref.to(y.dtype).double() - ref).norm()
     assert off <= 1.03 * least, float(off / least)
+
+
+@pytest.mark.parametrize("d,f", [(1001, 255), (1000, 255), (1001, 256)])
+def test_experts_one_token_reserves_room_for_its_experts_alone(cuda, d, f):
+    """Rows off 16 bytes (of both weights, of w_out, of w_in): 8 of 512 experts are copied, 13 MB of 786."""
+    import torch
+
+    from tpt_infer_b200 import CudaBackend
+
+    x, ids, wts, w_in, w_out = expert_inputs(1, 512, 8, d, f, "bf16", True)
+    run_experts(cuda, x, ids, wts, w_in, w_out, "silu", True, None, "bf16")  # the kernels are loaded
+    y = torch.empty_like(x)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    be = CudaBackend.new(0)
+    try:
+        be.experts_mlp_dev(x, ids, wts, w_in, w_out, 3, True, None, y)
+        be.sync()
+        assert free - torch.cuda.mem_get_info()[0] < 64 << 20
+        check(y, *want_experts(x, ids, wts, w_in, w_out, "silu", True, None, "bf16"))
+    finally:
+        be.close()

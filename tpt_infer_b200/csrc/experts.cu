@@ -491,7 +491,10 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
     size_t o_w[2] = {0, 0};
     for (int i = 0; i < 2; i++) {
         pad[i] = w_k[i] % 8 != 0 || !rows16_ok(w_src[i], w_k[i], experts * w_er[i]);
-        if (pad[i]) o_w[i] = take(experts * w_er[i] * up8(w_k[i]) * 2);
+        // the few-token kernels find the named experts by the order of their choice, so
+        // that one decoded token does not reserve room for every expert
+        const size_t room = stream && tokens * top_k < experts ? tokens * top_k : experts;
+        if (pad[i]) o_w[i] = take(room * w_er[i] * up8(w_k[i]) * 2);
     }
     const int planes = few ? 2 : 1;
     const size_t per_token = top_k * (planes * ldh * 2 + ldp * 4 + (gather ? 0 : lds * 2) + 8);
@@ -526,6 +529,7 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
         if (tokens * top_k <= 32) {
             job[i].ids = ids;
             job[i].pairs = (int)(tokens * top_k);
+            job[i].compact = stream;
         }
     }
     if (stream && !x_ok) job[2] = PadJob{x, ldx, tokens, d, ctx->ws + o_x, nullptr, 0, 1};
@@ -552,6 +556,8 @@ int run_experts(tpt_cuda_ctx *ctx, int dtype, const T *x, size_t ldx, size_t tok
     o.k = (int)f;
     o.experts = (int)experts;
     if (stream) {
+        g.compact = pad[0];
+        o.compact = pad[1];
         g.x = x_ok ? (const void *)x : (const void *)(ctx->ws + o_x);
         g.ldx = x_ok ? ldx : lds;
         g.x_rows = (int)tokens;

@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(256) k_pad_rows16(PadJob a, PadJob b, PadJob c
     const size_t all = job == 0 ? a.rows : job == 1 ? b.rows : c.rows;
     const size_t er = job == 0 ? a.expert_rows : job == 1 ? b.expert_rows : c.expert_rows;
     const int pairs = job == 0 ? a.pairs : job == 1 ? b.pairs : c.pairs;
+    const bool compact = job == 0 ? a.compact : job == 1 ? b.compact : c.compact;
     size_t rows = all;
     int id = -1;
     unsigned firsts = 0;
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(256) k_pad_rows16(PadJob a, PadJob b, PadJob c
             r = (size_t)__shfl_sync(0xffffffffu, id, __fns(firsts, 0, tile + 1)) * er + (i - tile * er);
         }
         const uintptr_t row = first + r * ld * 2, base = row & ~(uintptr_t)15;
-        uint4 *out = static_cast<uint4 *>(dst) + r * pieces;
+        uint4 *out = static_cast<uint4 *>(dst) + (compact ? i : r) * pieces;
         if (base >= first && base + (pieces + 1) * 16 <= last)
             pad_row<true>(first, last, row, k, pieces, out, lane);
         else

@@ -34,6 +34,7 @@ struct Gemm16 {
     int rows = 0, n = 0, k = 0;    // rows of X (dense) or slots (grouped); output features; products per output
     int x_rows = 0;                // rows that X has in memory
     int experts = 1;
+    bool compact = false;  // w holds only the experts that the call names, in the order of their first choice
     const int *row_token = nullptr;
     const Tile16 *tiles = nullptr;
     const int *n_tiles = nullptr;
@@ -82,7 +83,8 @@ inline bool rows16_ok(const void *p, size_t ld, size_t rows) {
 }
 // dst [rows][k rounded up to a multiple of 8, at least 8] = src [rows][k],
 // zero-filled; three of them in one launch. With ids only the rows of the experts
-// that they name are copied (up to 32 pairs, expert_rows rows an expert).
+// that they name are copied (up to 32 pairs, expert_rows rows an expert), to their own
+// places or, compact, one after the other in the order of their first choice.
 struct PadJob {
     const void *src = nullptr;
     size_t ld = 0, rows = 0, k = 0;
@@ -90,6 +92,7 @@ struct PadJob {
     const int *ids = nullptr;
     int pairs = 0;
     size_t expert_rows = 1;
+    bool compact = false;
 };
 int launch_pad_rows16(tpt_cuda_ctx *ctx, const PadJob &a, const PadJob &b, const PadJob &c);
 

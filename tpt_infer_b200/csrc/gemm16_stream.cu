@@ -35,6 +35,7 @@ struct StreamArgs {
     const int *ids;
     const float *weights;
     int pairs, top_k, experts;
+    int compact;  // w has the tiles' experts only, in the order of the tiles
     const void *bias;
     int act;
     const void *residual;
@@ -129,7 +130,7 @@ __global__ void __launch_bounds__(ST_T, 2) k_gemm16_stream(const __grid_constant
         const unsigned firsts = __ballot_sync(0xffffffffu, valid && leader == lane);
         n_tiles = __popc(firsts);
         const int tile = __popc(firsts & ((1u << leader) - 1));
-        if (warp == 0 && valid && leader == lane) tile_expert[tile] = id;
+        if (warp == 0 && valid && leader == lane) tile_expert[tile] = a.compact ? tile : id;
         if (SUM) {
             // a token that chose the expert twice takes it once, with both weights
             const unsigned twin = __match_any_sync(0xffffffffu, valid ? id * 4 + tok : -1 - lane);
@@ -369,6 +370,7 @@ StreamArgs base_args(tpt_cuda_ctx *ctx, const Gemm16 &g) {
     a.w = g.w;
     a.ldw = g.ldw;
     a.w_expert = g.w_expert;
+    a.compact = g.compact;
     a.n = g.n;
     a.k = g.k;
     a.bias = g.bias;
