@@ -998,9 +998,11 @@ int launch_split(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
 
 template <typename T, typename TY, bool GATED, int NT, bool LOW = false>
 int launch_split_k(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g, int ks) {
+    if constexpr (NT < 128) {  // the wide tile's k is split over 4 CTAs at most (launch_tc)
+        if (ks == 8) return launch_split<T, TY, GATED, NT, 8, LOW>(ctx, dtype, g);
+        if (ks == 6) return launch_split<T, TY, GATED, NT, 6, LOW>(ctx, dtype, g);
+    }
     switch (ks) {
-        case 8: return launch_split<T, TY, GATED, NT, 8, LOW>(ctx, dtype, g);
-        case 6: return launch_split<T, TY, GATED, NT, 6, LOW>(ctx, dtype, g);
         case 4: return launch_split<T, TY, GATED, NT, 4, LOW>(ctx, dtype, g);
         case 3: return launch_split<T, TY, GATED, NT, 3, LOW>(ctx, dtype, g);
         case 2: return launch_split<T, TY, GATED, NT, 2, LOW>(ctx, dtype, g);
@@ -1032,9 +1034,11 @@ int launch_tc(tpt_cuda_ctx *ctx, int dtype, const Gemm16 &g) {
     if constexpr (!GATED && std::is_same<TY, float>::value)
         if (g.x_low) return launch_split_k<T, TY, GATED, 16, true>(ctx, dtype, g, ks);  // tiles of 16: the caller's choice
     if (nt == 16) return launch_split_k<T, TY, GATED, 16>(ctx, dtype, g, ks);
-    if (nt == 32) return launch_split_k<T, TY, GATED, 32>(ctx, dtype, g, ks);
-    if (nt == 64) return launch_split_k<T, TY, GATED, 64>(ctx, dtype, g, ks);
-    return launch_split_k<T, TY, GATED, 128>(ctx, dtype, g, ks);
+    if constexpr (!GATED) {  // gated products are the experts', in tiles of 16, 32 or 256
+        if (nt == 64) return launch_split_k<T, TY, GATED, 64>(ctx, dtype, g, ks);
+        if (nt == 128) return launch_split_k<T, TY, GATED, 128>(ctx, dtype, g, ks);
+    }
+    return launch_split_k<T, TY, GATED, 32>(ctx, dtype, g, ks);
 }
 
 template <typename T>
