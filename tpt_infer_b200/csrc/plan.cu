@@ -423,6 +423,10 @@ int tpt_cuda_plan_add_op(tpt_cuda_plan *p, const tpt_plan_op *op) {
     if ((op->in1 >= 0 && !valid_id(p, op->in1)) || (op->in2 >= 0 && !valid_id(p, op->in2))) return TPT_INVALID;
     if (op->kind == TPT_OP_LINEAR_W8A8 && (!op->w || op->w->kind != 8)) return TPT_INVALID;
     if (op->kind < TPT_OP_QUANTIZE || op->kind > TPT_OP_BATCHED_MATMUL) return TPT_UNSUPPORTED;
+    // the epilogues of a plan know tpt_act up to gelu; silu is the 16-bit products' alone
+    const bool has_act = op->kind == TPT_OP_LINEAR_W8A8 || op->kind == TPT_OP_MATMUL_F32 ||
+                         op->kind == TPT_OP_BIAS_ACT || op->kind == TPT_OP_ADD_ACT;
+    if (has_act && (op->act < TPT_ACT_NONE || op->act > TPT_ACT_GELU)) return TPT_INVALID;
     if (op->kind >= TPT_OP_BINARY) {
         const int st = validate_graph_op(p, *op);
         if (st) return st;
