@@ -63,7 +63,9 @@ __device__ __forceinline__ void pad_row(uintptr_t first, uintptr_t last, uintptr
 }
 
 // blockIdx.y: the operand; a warp per row. Bound by the bytes read and written (1003 and
-// 1537 rows of 2051: 21 MB, ~5 us, from L2 in part).
+// 1537 rows of 2051: 21 MB, ~5 us, from L2 in part). COMPACT: the jobs with ids are compact
+// (a template argument: chosen at run time it cost 8 registers and 0.2 us everywhere).
+template <bool COMPACT>
 __global__ void __launch_bounds__(256) k_pad_rows16(PadJob a, PadJob b, PadJob c) {
     pdl_wait();
     pdl_trigger();
@@ -75,7 +77,6 @@ __global__ void __launch_bounds__(256) k_pad_rows16(PadJob a, PadJob b, PadJob c
     const size_t all = job == 0 ? a.rows : job == 1 ? b.rows : c.rows;
     const size_t er = job == 0 ? a.expert_rows : job == 1 ? b.expert_rows : c.expert_rows;
     const int pairs = job == 0 ? a.pairs : job == 1 ? b.pairs : c.pairs;
-    const bool compact = job == 0 ? a.compact : job == 1 ? b.compact : c.compact;
     size_t rows = all;
     int id = -1;
     unsigned firsts = 0;
@@ -96,7 +97,7 @@ __global__ void __launch_bounds__(256) k_pad_rows16(PadJob a, PadJob b, PadJob c
             r = (size_t)__shfl_sync(0xffffffffu, id, __fns(firsts, 0, tile + 1)) * er + (i - tile * er);
         }
         const uintptr_t row = first + r * ld * 2, base = row & ~(uintptr_t)15;
-        uint4 *out = static_cast<uint4 *>(dst) + (compact ? i : r) * pieces;
+        uint4 *out = static_cast<uint4 *>(dst) + (COMPACT ? i : r) * pieces;
         if (base >= first && base + (pieces + 1) * 16 <= last)
             pad_row<true>(first, last, row, k, pieces, out, lane);
         else
@@ -113,7 +114,8 @@ int launch_pad_rows16(tpt_cuda_ctx *ctx, const PadJob &a, const PadJob &b, const
         const size_t named = j->pairs * j->expert_rows, rows = j->ids && named < j->rows ? named : j->rows;
         if (rows > most) most = rows;
     }
-    launch_pdl(k_pad_rows16, dim3(grid_1d(most, 8, (unsigned)ctx->sm_count * 8), c.rows ? 3 : b.rows ? 2 : 1), 256, 0,
+    auto kern = a.compact || b.compact ? k_pad_rows16<true> : k_pad_rows16<false>;
+    launch_pdl(kern, dim3(grid_1d(most, 8, (unsigned)ctx->sm_count * 8), c.rows ? 3 : b.rows ? 2 : 1), 256, 0,
                ctx->stream, a, b, c);
     return after_launch(ctx, "pad_rows16");
 }
