@@ -14,7 +14,7 @@
 //                   clocks, 555 us = 1330 where the power limit holds them)
 //   k_gemm16_split  128 weight rows x up to 128 tokens per SM, k split over a
 //                   cluster, for work bound by the weights' stream
-//                   (64 x 4096 x 11008: 92 MB in 21.3 us = 4.3 TB/s)
+//                   (64 x 4096 x 11008: 92 MB in 21.5 us = 4.3 TB/s)
 //
 // Gated layers: each 32-lane quarter holds 16 gate rows and the 16 up rows of
 // the same features (one TMA box over the two halves of W), so the two meet
